@@ -343,6 +343,68 @@ int i8l_add_rmsnorm_quant_mm(const void* x, const void* residual, const void* we
  * host-only. */
 int i8l_add_rmsnorm_quant_mm_supported(int64_t M, int64_t N, int64_t K, const i8l_config* cfg);
 
+/*
+ * MXFP4 (OCP microscaling) operators.  An MXFP4 matrix [R,K] is E2M1 codes [R,K/2] (a byte holds
+ * elements 2i in its low and 2i+1 in its high nibble) and one E8M0 scale byte for each 32
+ * elements of a row [R,K/32]: 2^(byte - 127), 255 meaning NaN.  K is a multiple of 32; anything
+ * else is I8L_INVALID_ARG.  No counterpart in the reference, whose linears are int8.
+ *
+ * i8l_mxfp4_quant: x [M,K] of x_dtype (bf16/f16/f32), rows ldx elements apart, to contiguous codes
+ * and scales.  The scale of a block whose largest magnitude is p is 2^(floor(log2 p) - 2), at
+ * least 2^-127; with round_scale, p is first rounded to E2M1's precision (peaks from 1.75 * 2^e
+ * take the next scale, so nothing saturates by more than a rounding).  Elements are rounded to
+ * nearest even and saturate at 6.  A block with an infinity or a NaN gets scale 255, codes 0.
+ */
+int i8l_mxfp4_quant(const void* x, int64_t ldx, uint8_t* q, uint8_t* scale, int64_t M, int64_t K,
+                    int32_t x_dtype, int32_t round_scale, void* stream);
+
+/* The values an MXFP4 matrix stands for, into a contiguous 16-byte aligned out [M,K] (bf16, f16 or
+ * f32; exact but for f16's range).  ldq and lds: bytes from a row of codes / scales to the next. */
+int i8l_mxfp4_dequant(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, void* out,
+                      int64_t M, int64_t K, int32_t out_dtype, void* stream);
+
+/* i8l_add_rmsnorm_quant with MXFP4 codes: the normalized row (the same values) is quantized as
+ * i8l_mxfp4_quant does.  residual and residual_out are both NULL or both given.  H up to 32768. */
+int i8l_add_rmsnorm_mxfp4_quant(const void* x, const void* residual, const void* weight, float eps,
+                                uint8_t* q, uint8_t* scale, void* residual_out, int64_t M,
+                                int64_t H, int32_t act_dtype, int32_t w_dtype, int32_t round_scale,
+                                void* stream);
+
+/* i8l_silu_mul_quant (round_silu) with MXFP4 codes: gate_up [M,2I] contiguous, silu rounded to
+ * act_dtype, its product with up rounded again, quantized as i8l_mxfp4_quant does. */
+int i8l_silu_mul_mxfp4_quant(const void* gate_up, uint8_t* q, uint8_t* scale, int64_t M, int64_t I,
+                             int32_t act_dtype, int32_t round_scale, void* stream);
+
+/*
+ * out[m,n] = cast(sum_k A[m,k] B[n,k] (+ bias[n])), A [M,K] and B [N,K] MXFP4, accumulated in
+ * fp32, one rounding to out_dtype (bf16/f16/f32).  lda, ldb, ldsa, ldsb: bytes from a row of codes
+ * or scales to the next; ldc in elements.  bias [N] (bf16/f16/f32) or NULL.  Any alignment; 16-byte
+ * aligned rows of codes are the fast ones.  Nothing is allocated.
+ */
+int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
+                 const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b, int64_t ldsb,
+                 const void* bias, int32_t bias_dtype, void* out, int64_t ldc, int32_t out_dtype,
+                 int64_t M, int64_t N, int64_t K, void* stream);
+
+/*
+ * RMSNorm of every query and key head and the rotation of its first R values by the token's
+ * position, in fp32 with one rounding:
+ *   h = x * rsqrt(mean(x^2) + eps) * w;  (h_a, h_b) -> (h_a c - h_b s, h_b c + h_a s)
+ * for the pairs (i, i + R/2), or (2i, 2i + 1) with interleaved.  q [T,Hq,D] and k [T,Hk,D] of
+ * act_dtype (bf16/f16), token and head strides in elements, values contiguous; the outputs likewise
+ * and may be the inputs themselves (same pointer and strides), else must not overlap them.
+ * q_weight and k_weight [D] of w_dtype, or NULL for none.  cos_sin [max_pos,R] of cs_dtype: the
+ * cosines of the R/2 frequencies, then their sines.  positions [T], pos_bits 32 or 64; a token
+ * whose position is outside [0, max_pos) gets NaN in its rotated values.
+ */
+int i8l_qk_norm_rope(const void* q, int64_t q_ts, int64_t q_hs, const void* k, int64_t k_ts,
+                     int64_t k_hs, void* q_out, int64_t qo_ts, int64_t qo_hs, void* k_out,
+                     int64_t ko_ts, int64_t ko_hs, const void* q_weight, const void* k_weight,
+                     int32_t w_dtype, float eps, const void* cos_sin, int32_t cs_dtype,
+                     int64_t max_pos, const void* positions, int32_t pos_bits, int64_t T,
+                     int64_t Hq, int64_t Hk, int64_t D, int64_t R, int32_t interleaved,
+                     int32_t act_dtype, void* stream);
+
 /* Thread-local description of the last failure ("" if none). */
 const char* i8l_last_error(void);
 

@@ -1,0 +1,32 @@
+// Internal interface of the MXFP4 product: its operands, the epilogue and the schedules.
+//
+//   out[m,n] = cast( sum_b 2^(sa[m,b]+sb[n,b]-254) sum_{i in block b} A[m,i] B[n,i]  (+ bias[n]) )
+//
+// A [M,K] and B [N,K] hold E2M1 codes, two a byte, sa [M,K/32] and sb [N,K/32] their E8M0 scales;
+// the sum is held in fp32 (a block's 32 products are multiples of 1/4 below 2^11: exact), the bias
+// is added in fp32 and the result rounded once.
+#pragma once
+
+#include "i8l_gemm.h"
+#include "i8l_mxfp4.h"
+
+namespace i8l {
+
+struct MxMM {
+  const uint8_t *a, *b, *sa, *sb;
+  int64_t lda, ldb, ldsa, ldsb;   // bytes from a row to the next
+  const void* bias;
+  void* out;
+  int64_t ldc;                    // elements
+  int64_t M, N, K;                // K in elements
+  int bias_dtype, out_dtype;
+};
+
+__device__ __forceinline__ void mx_store(const MxMM& p, int64_t m, int64_t n, float v) {
+  const int64_t at = m * p.ldc + n;
+  if (p.out_dtype == I8L_F32) ((float*)p.out)[at] = v;
+  else if (p.out_dtype == I8L_BF16) ((uint16_t*)p.out)[at] = f32_to_bf16_bits(v);
+  else ((uint16_t*)p.out)[at] = f32_to_f16_bits(v);
+}
+
+}  // namespace i8l

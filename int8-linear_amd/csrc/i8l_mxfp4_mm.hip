@@ -1,0 +1,83 @@
+// The MXFP4 product: the kernel for any strides and alignment, the choice of schedule and the C
+// entry point.
+#include "i8l_mxfp4_mm.h"
+
+namespace i8l {
+
+namespace {
+
+// One thread an output, a block of 32 at a time: the block's exact sum, then one scaled addition.
+__global__ void __launch_bounds__(256) mxfp4_mm_any(MxMM p) {
+  const int64_t n = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int64_t m = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (m >= p.M || n >= p.N) return;
+  const uint8_t *a = p.a + m * p.lda, *b = p.b + n * p.ldb;
+  const uint8_t *sa = p.sa + m * p.ldsa, *sb = p.sb + n * p.ldsb;
+  float acc = 0.0f;
+  for (int64_t blk = 0; blk < p.K / kMxBlock; ++blk) {
+    float s = 0.0f;
+    for (int i = 0; i < kMxBlock / 2; ++i) {
+      const uint32_t x = a[blk * 16 + i], y = b[blk * 16 + i];
+      s += e2m1_value(x & 15) * e2m1_value(y & 15) + e2m1_value(x >> 4) * e2m1_value(y >> 4);
+    }
+    const int ea = sa[blk], eb = sb[blk];
+    acc += ea == 255 || eb == 255 ? __builtin_nanf("") : __builtin_ldexpf(s, ea + eb - 254);
+  }
+  if (p.bias) acc += load_bias(p.bias, p.bias_dtype, n);
+  mx_store(p, m, n, acc);
+}
+
+hipError_t launch_mx_any(const MxMM& p, hipStream_t st) {
+  // the grid's y counts up to 65535: longer batches in pieces
+  const int64_t most = 65535 * 4;
+  for (int64_t m = 0; m < p.M; m += most) {
+    MxMM q = p;
+    q.M = std::min(most, p.M - m);
+    q.a += m * p.lda;
+    q.sa += m * p.ldsa;
+    q.out = (char*)p.out + m * p.ldc * elt_size(p.out_dtype);
+    hipLaunchKernelGGL(mxfp4_mm_any, dim3((unsigned)((p.N + 63) / 64), (unsigned)((q.M + 3) / 4)),
+                       dim3(256), 0, st, q);
+    if (const hipError_t e = hipGetLastError()) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace
+}  // namespace i8l
+
+using namespace i8l;
+
+extern "C" int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
+                            const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b,
+                            int64_t ldsb, const void* bias, int32_t bias_dtype, void* out,
+                            int64_t ldc, int32_t out_dtype, int64_t M, int64_t N, int64_t K,
+                            void* stream) {
+  if (M < 0 || N < 0 || K <= 0 || K % kMxBlock) {
+    set_error("mxfp4_mm: bad sizes M=%lld N=%lld K=%lld (K in whole blocks of 32)", (long long)M,
+              (long long)N, (long long)K);
+    return I8L_INVALID_ARG;
+  }
+  auto float_dt = [](int dt) { return dt == I8L_BF16 || dt == I8L_F16 || dt == I8L_F32; };
+  if (!float_dt(out_dtype) || (bias && !float_dt(bias_dtype))) {
+    set_error("mxfp4_mm: the output and the bias must be bf16, fp16 or fp32");
+    return I8L_UNSUPPORTED;
+  }
+  if (M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) {
+    set_error("mxfp4_mm: M=%lld N=%lld K=%lld: too large", (long long)M, (long long)N, (long long)K);
+    return I8L_UNSUPPORTED;
+  }
+  const int64_t kb = K / 2, ks = K / kMxBlock;
+  if ((M > 1 && (lda < kb || ldsa < ks || ldc < N)) || (N > 1 && (ldb < kb || ldsb < ks))) {
+    set_error("mxfp4_mm: a row stride is shorter than its row (a %lld, b %lld, scales %lld and "
+              "%lld, out %lld for M=%lld N=%lld K=%lld)", (long long)lda, (long long)ldb,
+              (long long)ldsa, (long long)ldsb, (long long)ldc, (long long)M, (long long)N,
+              (long long)K);
+    return I8L_INVALID_ARG;
+  }
+  if (M == 0 || N == 0) return I8L_OK;
+  if (!operands_ok("mxfp4_mm", {a, b, scale_a, scale_b, out})) return I8L_INVALID_ARG;
+  const MxMM p{a, b, scale_a, scale_b, lda, ldb, ldsa, ldsb, bias, out, ldc, M, N, K,
+               bias ? bias_dtype : I8L_DTYPE_NONE, out_dtype};
+  return hip_status(launch_mx_any(p, (hipStream_t)stream), "mxfp4_mm launch");
+}

@@ -254,6 +254,174 @@ py::object quant_per_token(const at::Tensor& x, bool precise_div) {
   return py::make_tuple(q, s);
 }
 
+// ------------------------------------------------------------------ MXFP4 and the q/k norm
+// Codes [R, K/2] and scales [R, K/32] as the kernels read them without a copy: uint8, unit stride
+// along K, rows that do not share memory.
+bool mx_plain(const at::Tensor& q, const at::Tensor& s, const at::Device& dev) {
+  if (q.dim() != 2 || s.dim() != 2 || q.scalar_type() != at::kByte || s.scalar_type() != at::kByte ||
+      q.device() != dev || s.device() != dev)
+    return false;
+  const int64_t r = q.size(0), kb = q.size(1);
+  if (kb == 0 || kb % 16 || s.size(0) != r || s.size(1) != kb / 16) return false;
+  return q.stride(1) == 1 && (s.stride(1) == 1 || s.size(1) == 1) &&
+         (r <= 1 || (q.stride(0) >= kb && s.stride(0) >= kb / 16));
+}
+
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+py::object mxfp4_quant(const at::Tensor& x, bool round_scale) {
+  if (x.dim() != 2 || !x.is_cuda()) return py::none();
+  const int64_t M = x.size(0), K = x.size(1);
+  const int32_t code = float_code(x.scalar_type());
+  if (code < 0 || K == 0 || K % 32 || x.stride(1) != 1 || (M > 1 && x.stride(0) < K))
+    return py::none();
+  at::Tensor q = empty_like_on(x, {M, K / 2}, at::kByte);
+  at::Tensor s = empty_like_on(x, {M, K / 32}, at::kByte);
+  const c10::DeviceGuard guard(x.device());
+  const int st = i8l_mxfp4_quant(x.data_ptr(), row_stride(x), (uint8_t*)q.data_ptr(),
+                                 (uint8_t*)s.data_ptr(), M, K, code, round_scale ? 1 : 0,
+                                 stream_of(x));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::make_tuple(q, s);
+}
+
+py::object mxfp4_dequant(const at::Tensor& q, const at::Tensor& s, at::ScalarType out_dtype) {
+  const int32_t code = float_code(out_dtype);
+  if (code < 0 || !q.is_cuda() || !mx_plain(q, s, q.device())) return py::none();
+  const int64_t M = q.size(0), K = 2 * q.size(1);
+  at::Tensor out = empty_like_on(q, {M, K}, out_dtype);
+  const c10::DeviceGuard guard(q.device());
+  const int st = i8l_mxfp4_dequant((const uint8_t*)q.data_ptr(), row_stride(q),
+                                   (const uint8_t*)s.data_ptr(), row_stride(s), out.data_ptr(), M,
+                                   K, code, stream_of(q));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::cast(out);
+}
+
+py::object add_rmsnorm_mxfp4_quant(const at::Tensor& x, const c10::optional<at::Tensor>& residual,
+                                   const at::Tensor& w, double eps, bool round_scale) {
+  if (x.dim() != 2 || !x.is_cuda() || !x.is_contiguous()) return py::none();
+  const int32_t act = act_code(x.scalar_type()), wcode = act_code(w.scalar_type());
+  const int64_t M = x.size(0), H = x.size(1);
+  if (act < 0 || wcode < 0 || H == 0 || H % 32 || w.numel() != H || w.device() != x.device() ||
+      !w.is_contiguous())
+    return py::none();
+  at::Tensor rout;
+  const void* rptr = nullptr;
+  if (residual.has_value()) {
+    const at::Tensor& r = *residual;
+    if (!r.is_contiguous() || r.sizes() != x.sizes() || r.scalar_type() != x.scalar_type() ||
+        r.device() != x.device())
+      return py::none();
+    rptr = r.data_ptr();
+    rout = empty_like_on(x, x.sizes(), x.scalar_type());
+  }
+  at::Tensor q = empty_like_on(x, {M, H / 2}, at::kByte);
+  at::Tensor s = empty_like_on(x, {M, H / 32}, at::kByte);
+  const c10::DeviceGuard guard(x.device());
+  const int st = i8l_add_rmsnorm_mxfp4_quant(
+      x.data_ptr(), rptr, w.data_ptr(), (float)eps, (uint8_t*)q.data_ptr(), (uint8_t*)s.data_ptr(),
+      rout.defined() ? rout.data_ptr() : nullptr, M, H, act, wcode, round_scale ? 1 : 0,
+      stream_of(x));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::make_tuple(q, s, rout.defined() ? py::cast(rout) : py::none());
+}
+
+py::object silu_mul_mxfp4_quant(const at::Tensor& gu, bool round_scale) {
+  if (gu.dim() != 2 || !gu.is_cuda() || !gu.is_contiguous() || gu.size(1) % 64 || !gu.size(1))
+    return py::none();
+  const int32_t act = act_code(gu.scalar_type());
+  if (act < 0) return py::none();
+  const int64_t M = gu.size(0), I = gu.size(1) / 2;
+  at::Tensor q = empty_like_on(gu, {M, I / 2}, at::kByte);
+  at::Tensor s = empty_like_on(gu, {M, I / 32}, at::kByte);
+  const c10::DeviceGuard guard(gu.device());
+  const int st = i8l_silu_mul_mxfp4_quant(gu.data_ptr(), (uint8_t*)q.data_ptr(),
+                                          (uint8_t*)s.data_ptr(), M, I, act, round_scale ? 1 : 0,
+                                          stream_of(gu));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::make_tuple(q, s);
+}
+
+py::object mxfp4_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa,
+                    const at::Tensor& sb, at::ScalarType out_dtype,
+                    const c10::optional<at::Tensor>& bias) {
+  const int32_t out_code = float_code(out_dtype);
+  if (out_code < 0 || !a.is_cuda() || a.dim() != 2 || b.dim() != 2 || a.size(1) != b.size(0))
+    return py::none();
+  const at::Device dev = a.device();
+  if (!mx_plain(a, sa, dev) || !mx_plain(b.t(), sb, dev)) return py::none();
+  const int64_t M = a.size(0), N = b.size(1), K = 2 * a.size(1);
+  int32_t bias_code = I8L_DTYPE_NONE;
+  const void* bias_ptr = nullptr;
+  if (bias.has_value()) {
+    const at::Tensor& bt = *bias;
+    bias_code = float_code(bt.scalar_type());
+    if (bias_code < 0 || bt.dim() != 1 || bt.size(0) != N || bt.device() != dev ||
+        !bt.is_contiguous())
+      return py::none();
+    bias_ptr = bt.data_ptr();
+  }
+  at::Tensor out = empty_like_on(a, {M, N}, out_dtype);
+  const c10::DeviceGuard guard(dev);
+  const int st = i8l_mxfp4_mm((const uint8_t*)a.data_ptr(), row_stride(a),
+                              (const uint8_t*)b.data_ptr(), N > 1 ? b.stride(1) : K / 2,
+                              (const uint8_t*)sa.data_ptr(), row_stride(sa),
+                              (const uint8_t*)sb.data_ptr(), row_stride(sb), bias_ptr, bias_code,
+                              out.data_ptr(), N, out_code, M, N, K, stream_of(a));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::cast(out);
+}
+
+py::object qk_norm_rope(const at::Tensor& q, const at::Tensor& k,
+                        const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw,
+                        const at::Tensor& cs, const at::Tensor& pos, double eps, bool interleaved,
+                        bool inplace) {
+  // (in place goes the Python way, which checks that the heads do not overlap)
+  if (inplace || !q.is_cuda() || q.dim() != 3 || k.dim() != 3 || q.size(0) != k.size(0) ||
+      q.size(2) != k.size(2) || k.scalar_type() != q.scalar_type() || q.size(2) < 2 ||
+      q.stride(2) != 1 || k.stride(2) != 1)
+    return py::none();
+  const at::Device dev = q.device();
+  const int32_t act = act_code(q.scalar_type());
+  const int64_t T = q.size(0), D = q.size(2);
+  if (act < 0 || k.device() != dev || cs.device() != dev || pos.device() != dev) return py::none();
+  int32_t wcode = I8L_DTYPE_NONE;
+  for (const auto* w : {&qw, &kw})
+    if (w->has_value()) {
+      const at::Tensor& t = **w;
+      const int32_t c = float_code(t.scalar_type());
+      if (c < 0 || (wcode != I8L_DTYPE_NONE && c != wcode) || t.dim() != 1 || t.size(0) != D ||
+          t.device() != dev || !t.is_contiguous())
+        return py::none();
+      wcode = c;
+    }
+  const int32_t cs_code = float_code(cs.scalar_type());
+  if (cs_code < 0 || cs.dim() != 2 || !cs.is_contiguous() || cs.size(1) % 2 || cs.size(1) > D ||
+      pos.dim() != 1 || pos.size(0) != T || !pos.is_contiguous())
+    return py::none();
+  const int32_t bits = pos.scalar_type() == at::kLong ? 64 : pos.scalar_type() == at::kInt ? 32 : 0;
+  if (!bits) return py::none();
+  const int64_t Hq = q.size(1), Hk = k.size(1);
+  at::Tensor qo = empty_like_on(q, {T, Hq, D}, q.scalar_type());
+  at::Tensor ko = empty_like_on(q, {T, Hk, D}, q.scalar_type());
+  const c10::DeviceGuard guard(dev);
+  const int st = i8l_qk_norm_rope(
+      q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), qo.data_ptr(),
+      Hq * D, D, ko.data_ptr(), Hk * D, D, qw.has_value() ? qw->data_ptr() : nullptr,
+      kw.has_value() ? kw->data_ptr() : nullptr, wcode, (float)eps, cs.data_ptr(), cs_code,
+      cs.size(0), pos.data_ptr(), bits, T, Hq, Hk, D, cs.size(1), interleaved ? 1 : 0, act,
+      stream_of(q));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::make_tuple(qo, ko);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_i8l_fast, m) {
@@ -268,4 +436,10 @@ PYBIND11_MODULE(_i8l_fast, m) {
   m.def("add_rmsnorm_quant", &add_rmsnorm_quant);
   m.def("silu_mul_quant", &silu_mul_quant);
   m.def("quant_per_token", &quant_per_token);
+  m.def("mxfp4_quant", &mxfp4_quant);
+  m.def("mxfp4_dequant", &mxfp4_dequant);
+  m.def("add_rmsnorm_mxfp4_quant", &add_rmsnorm_mxfp4_quant);
+  m.def("silu_mul_mxfp4_quant", &silu_mul_mxfp4_quant);
+  m.def("mxfp4_mm", &mxfp4_mm);
+  m.def("qk_norm_rope", &qk_norm_rope);
 }

@@ -36,8 +36,9 @@ EXPORTS = ("i8l_w8a8_mm", "i8l_w8a8_mm_supported", "i8l_default_config", "i8l_la
            "i8l_silu_mul_quant_mm", "i8l_silu_mul_quant_mm_supported", "i8l_w8a8_mm_ws",
            "i8l_w8a8_mm_workspace_bytes", "i8l_w8a8_mm_noalloc", "i8l_init",
            "i8l_add_rmsnorm_quant_mm", "i8l_add_rmsnorm_quant_mm_supported",
-           "i8l_w8a8_mm_silu_mul", "i8l_w8a8_mm_silu_mul_supported", "i8l_last_error",
-           "i8l_version")
+           "i8l_w8a8_mm_silu_mul", "i8l_w8a8_mm_silu_mul_supported", "i8l_mxfp4_quant",
+           "i8l_mxfp4_dequant", "i8l_add_rmsnorm_mxfp4_quant", "i8l_silu_mul_mxfp4_quant",
+           "i8l_mxfp4_mm", "i8l_qk_norm_rope", "i8l_last_error", "i8l_version")
 
 _lib: ctypes.CDLL | None = None
 
@@ -82,6 +83,16 @@ def lib() -> ctypes.CDLL:
                                        _P, _I64, _I32, _I64, _I64, _I64,
                                        ctypes.POINTER(CConfig), _P]
     L.i8l_w8a8_mm_silu_mul_supported.argtypes = [_I64, _I64, _I64, ctypes.POINTER(CConfig)]
+    L.i8l_mxfp4_quant.argtypes = [_P, _I64, _P, _P, _I64, _I64, _I32, _I32, _P]
+    L.i8l_mxfp4_dequant.argtypes = [_P, _I64, _P, _I64, _P, _I64, _I64, _I32, _P]
+    L.i8l_add_rmsnorm_mxfp4_quant.argtypes = [_P, _P, _P, ctypes.c_float, _P, _P, _P, _I64, _I64,
+                                              _I32, _I32, _I32, _P]
+    L.i8l_silu_mul_mxfp4_quant.argtypes = [_P, _P, _P, _I64, _I64, _I32, _I32, _P]
+    L.i8l_mxfp4_mm.argtypes = [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I32, _P, _I64, _I32,
+                               _I64, _I64, _I64, _P]
+    L.i8l_qk_norm_rope.argtypes = [_P, _I64, _I64] * 4 + [_P, _P, _I32, ctypes.c_float, _P, _I32,
+                                                          _I64, _P, _I32, _I64, _I64, _I64, _I64,
+                                                          _I64, _I32, _I32, _P]
     for name in EXPORTS[:-2]:
         getattr(L, name).restype = ctypes.c_int
     L.i8l_w8a8_mm_workspace_bytes.restype = _I64
