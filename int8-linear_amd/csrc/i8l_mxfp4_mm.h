@@ -29,4 +29,37 @@ __device__ __forceinline__ void mx_store(const MxMM& p, int64_t m, int64_t n, fl
   else ((uint16_t*)p.out)[at] = f32_to_f16_bits(v);
 }
 
+// Four neighbouring columns n .. n + 3 of row m (n a multiple of 4): the bias, one rounding, one
+// store where the columns and the alignment allow it.
+__device__ __forceinline__ void mx_store4(const MxMM& p, int64_t m, int64_t n, v4f v) {
+  if (n >= p.N) return;
+  const int es = p.out_dtype == I8L_F32 ? 4 : 2;
+  char* at = (char*)p.out + (m * p.ldc + n) * es;
+  if (n + 4 <= p.N) {
+    if (p.bias) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] += load_bias(p.bias, p.bias_dtype, n + r);
+    }
+    if (((uintptr_t)at & (4 * es - 1)) == 0) {
+      if (p.out_dtype == I8L_F32) *(v4f*)at = v;
+      else if (p.out_dtype == I8L_BF16)
+        *(uint2*)at = make_uint2(f32x2_to_act2<I8L_BF16>(v[0], v[1]), f32x2_to_act2<I8L_BF16>(v[2], v[3]));
+      else
+        *(uint2*)at = make_uint2(f32x2_to_act2<I8L_F16>(v[0], v[1]), f32x2_to_act2<I8L_F16>(v[2], v[3]));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx_store(p, m, n + r, v[r]);
+    }
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n + r < p.N)
+      mx_store(p, m, n + r, p.bias ? v[r] + load_bias(p.bias, p.bias_dtype, n + r) : v[r]);
+}
+
+// Few tokens, or sizes the macro tiles do not take (i8l_mxfp4_decode.hip): rows of codes on 16 bytes.
+bool mx_decode_ok(const MxMM& p);
+hipError_t launch_mx_decode(const MxMM& p, hipStream_t st);
+
 }  // namespace i8l

@@ -79,5 +79,7 @@ extern "C" int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int
   if (!operands_ok("mxfp4_mm", {a, b, scale_a, scale_b, out})) return I8L_INVALID_ARG;
   const MxMM p{a, b, scale_a, scale_b, lda, ldb, ldsa, ldsb, bias, out, ldc, M, N, K,
                bias ? bias_dtype : I8L_DTYPE_NONE, out_dtype};
-  return hip_status(launch_mx_any(p, (hipStream_t)stream), "mxfp4_mm launch");
+  const hipStream_t st = (hipStream_t)stream;
+  const hipError_t e = mx_decode_ok(p) ? launch_mx_decode(p, st) : launch_mx_any(p, st);
+  return hip_status(e, "mxfp4_mm launch");
 }
