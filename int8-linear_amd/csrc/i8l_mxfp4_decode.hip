@@ -1,4 +1,5 @@
-// MXFP4 product for few tokens: weights streamed once from memory into v_mfma_scale_f32_16x16x128.
+// MXFP4 product for a K of any whole blocks: operands straight from memory into
+// v_mfma_scale_f32_16x16x128.
 //
 // A workgroup covers 16 MT tokens and 16 NT columns; its W waves take the K steps of 512 elements
 // in turn (step s: wave s % W) and their partial sums are added through LDS in wave order.  In a
@@ -7,8 +8,9 @@
 // word u of the row's 16 scale bytes, which one load brings.  The weight is the first MFMA operand,
 // so a lane's four sums are four neighbouring columns of one token: one store.
 //
-// What bounds it: HBM, reading (1/2 + 1/32) N K bytes.  The activations come from L2, M K / 2
-// bytes a workgroup, which is why NT grows with the tokens.
+// What bounds it: cache lines, one a lane and load, as neighbouring lanes hold different rows (90
+// cycles a load instruction on a CU): 2752 -> 4096 at 1 token DECODE_1 us, at 64 DECODE_64.  The rows that
+// i8l_mxfp4_ring.hip takes go through LDS instead.
 #include "i8l_mxfp4_mm.h"
 
 namespace i8l {
@@ -129,7 +131,8 @@ hipError_t launch_decode_k(const MxMM& p, hipStream_t st) {
   auto kern = mxfp4_decode<MT, NT, W>;
   constexpr size_t shm = (size_t)W * MT * NT * 1024;
   static_assert(shm <= 64 * 1024, "the partial sums fit the LDS of any launch");
-  const dim3 grid((unsigned)((p.N + 16 * NT - 1) / (16 * NT)), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
+  const dim3 grid((unsigned)((p.N + 16 * NT - 1) / (16 * NT)),
+                  (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
   hipLaunchKernelGGL(kern, grid, dim3(64 * W), shm, st, p);
   return hipGetLastError();
 }
@@ -141,21 +144,15 @@ bool mx_decode_ok(const MxMM& p) {
          (p.M + 16 * kMaxMT - 1) / (16 * kMaxMT) <= 65535 && p.K <= (int64_t)kStep * INT32_MAX;
 }
 
-hipError_t launch_mx_decode_cfg(int mt, int nt, int w, const MxMM& p, hipStream_t st) {
-#define I8L_D(MT_, NT_, W_) \
-  if (mt == MT_ && nt == NT_ && w == W_) return launch_decode_k<MT_, NT_, W_>(p, st);
-#define I8L_DW(MT_, NT_) I8L_D(MT_, NT_, 4) I8L_D(MT_, NT_, 8)
-  I8L_DW(1, 1) I8L_DW(2, 1) I8L_DW(3, 1) I8L_DW(4, 1) I8L_DW(5, 1) I8L_DW(6, 1) I8L_DW(7, 1) I8L_DW(8, 1)
-  I8L_DW(1, 2) I8L_DW(2, 2) I8L_DW(3, 2) I8L_DW(4, 2) I8L_D(5, 2, 4) I8L_D(6, 2, 4) I8L_D(7, 2, 4) I8L_D(8, 2, 4)
-  I8L_D(1, 1, 16) I8L_D(2, 1, 16) I8L_D(3, 1, 16) I8L_D(4, 1, 16)
-#undef I8L_DW
-#undef I8L_D
-  return hipErrorInvalidValue;
-}
-
+// Eight waves; the tokens in as few tiles as hold them.
 hipError_t launch_mx_decode(const MxMM& p, hipStream_t st) {
-  const int mt = (int)std::min<int64_t>(kMaxMT, (p.M + 15) / 16);
-  return launch_mx_decode_cfg(mt, 1, 8, p, st);
+  switch (std::min<int64_t>(kMaxMT, (p.M + 15) / 16)) {
+    case 1: return launch_decode_k<1, 1, 8>(p, st);
+    case 2: return launch_decode_k<2, 1, 8>(p, st);
+    case 3:
+    case 4: return launch_decode_k<4, 1, 8>(p, st);
+  }
+  return launch_decode_k<kMaxMT, 1, 8>(p, st);
 }
 
 }  // namespace i8l

@@ -58,7 +58,14 @@ __device__ __forceinline__ void mx_store4(const MxMM& p, int64_t m, int64_t n, v
       mx_store(p, m, n + r, p.bias ? v[r] + load_bias(p.bias, p.bias_dtype, n + r) : v[r]);
 }
 
-// Few tokens, or sizes the macro tiles do not take (i8l_mxfp4_decode.hip): rows of codes on 16 bytes.
+// Many tokens (i8l_mxfp4_phased.hip): K in whole pairs of 256-element steps, everything on 16 bytes.
+bool mx_phased_ok(const MxMM& p);
+hipError_t launch_mx_phased(const MxMM& p, hipStream_t st);
+// Few tokens (i8l_mxfp4_ring.hip): whole 128-element runs of K, rows of codes on 16 bytes and of
+// scales on 4.
+bool mx_ring_ok(const MxMM& p);
+hipError_t launch_mx_ring(const MxMM& p, hipStream_t st);
+// Any whole blocks of K (i8l_mxfp4_decode.hip): rows of codes on 16 bytes.
 bool mx_decode_ok(const MxMM& p);
 hipError_t launch_mx_decode(const MxMM& p, hipStream_t st);
 

@@ -80,6 +80,9 @@ extern "C" int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int
   const MxMM p{a, b, scale_a, scale_b, lda, ldb, ldsa, ldsb, bias, out, ldc, M, N, K,
                bias ? bias_dtype : I8L_DTYPE_NONE, out_dtype};
   const hipStream_t st = (hipStream_t)stream;
-  const hipError_t e = mx_decode_ok(p) ? launch_mx_decode(p, st) : launch_mx_any(p, st);
+  const hipError_t e = p.M > 128 && mx_phased_ok(p) ? launch_mx_phased(p, st)
+                       : mx_ring_ok(p)              ? launch_mx_ring(p, st)
+                       : mx_decode_ok(p)            ? launch_mx_decode(p, st)
+                                                    : launch_mx_any(p, st);
   return hip_status(e, "mxfp4_mm launch");
 }

@@ -255,7 +255,8 @@ MS = [1, 2, 7, 16, 17, 33, 64, 65, 100, 128, 129, 257, 300]
 
 @pytest.mark.parametrize("m", MS)
 @pytest.mark.parametrize("n,k", [(64, 32), (1, 64), (5, 96), (130, 160), (257, 512), (96, 1056),
-                                 (512, 1024), (320, 2048), (192, 4096)])
+                                 (512, 1024), (320, 2048), (192, 4096), (96, 384), (4112, 128),
+                                 (64, 12544)])
 def test_mm_exact(m, n, k):
     _check_exact(m, n, k)
 
