@@ -386,6 +386,18 @@ int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
                  const void* bias, int32_t bias_dtype, void* out, int64_t ldc, int32_t out_dtype,
                  int64_t M, int64_t N, int64_t K, void* stream);
 
+/* The same with K split over workgroups where that is faster (some 100 to 512 tokens of a long K):
+ * the fp32 partial sums go to the caller's workspace, 16-byte aligned, of at least
+ * i8l_mxfp4_mm_workspace_bytes(M, N, K) bytes (0: the call never splits), and a second kernel adds
+ * them in order.  A NULL, misaligned or smaller workspace is not used.  Calls that overlap must not
+ * share one. */
+int i8l_mxfp4_mm_ws(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
+                    const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b, int64_t ldsb,
+                    const void* bias, int32_t bias_dtype, void* out, int64_t ldc, int32_t out_dtype,
+                    int64_t M, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+int64_t i8l_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K);
+
 /*
  * RMSNorm of every query and key head and the rotation of its first R values by the token's
  * position, in fp32 with one rounding:

@@ -59,8 +59,14 @@ __device__ __forceinline__ void mx_store4(const MxMM& p, int64_t m, int64_t n, v
 }
 
 // Many tokens (i8l_mxfp4_phased.hip): K in whole pairs of 256-element steps, everything on 16 bytes.
+// A workspace lets it split K: its plan never needs more than kMaxParts planes of M x N floats.
 bool mx_phased_ok(const MxMM& p);
-hipError_t launch_mx_phased(const MxMM& p, hipStream_t st);
+constexpr int kMaxParts = 8;
+struct MxPhasedPlan {
+  int tile, splits;
+};
+MxPhasedPlan mx_phased_plan(int64_t M, int64_t N, int64_t K, int64_t workspace);
+hipError_t launch_mx_phased(const MxMM& p, void* workspace, int64_t bytes, hipStream_t st);
 // Few tokens (i8l_mxfp4_ring.hip): whole 128-element runs of K, rows of codes on 16 bytes and of
 // scales on 4.
 bool mx_ring_ok(const MxMM& p);

@@ -43,16 +43,37 @@ hipError_t launch_mx_any(const MxMM& p, hipStream_t st) {
   return hipSuccess;
 }
 
+// Whether the macro tiles are faster than the ring, by tokens, the more the columns (each in us,
+// ring / tiles, cold weights): 28672 columns at 32 tokens 15.1 / 15.9 and at 48 18.5 / 16.5; 12288 at
+// 64 7.9 / 8.4 and at 80 9.2 / 8.6; 6144 at 128 11.3 / 14.7; and where a long K is split, 14336 -> 4096
+// at 80 15.8 / 16.1 and at 96 18.1 / 16.7 (6144 -> 2048 at 128 11.6 / 12.8).
+bool many_tokens(int64_t M, int64_t N, int64_t K, bool split) {
+  return M > (N >= 20480 ? 32 : N >= 9216 ? 72 : split && K >= 8192 ? 80 : 128);
+}
+
+constexpr int64_t kMostWorkspace = (int64_t)64 << 20;
+
+// The sizes alone of mx_phased_ok.
+bool phased_sizes(int64_t M, int64_t N, int64_t K) {
+  return M > 0 && N >= 128 && N % 8 == 0 && K >= 1024 && K % 512 == 0;
+}
+
 }  // namespace
 }  // namespace i8l
 
 using namespace i8l;
 
-extern "C" int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
-                            const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b,
-                            int64_t ldsb, const void* bias, int32_t bias_dtype, void* out,
-                            int64_t ldc, int32_t out_dtype, int64_t M, int64_t N, int64_t K,
-                            void* stream) {
+extern "C" int64_t i8l_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (!phased_sizes(M, N, K) || M > 4096 || N > INT32_MAX || K > INT32_MAX) return 0;
+  const int splits = mx_phased_plan(M, N, K, kMostWorkspace).splits;
+  return splits > 1 && many_tokens(M, N, K, true) ? splits * M * N * 4 : 0;
+}
+
+extern "C" int i8l_mxfp4_mm_ws(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
+                               const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b,
+                               int64_t ldsb, const void* bias, int32_t bias_dtype, void* out,
+                               int64_t ldc, int32_t out_dtype, int64_t M, int64_t N, int64_t K,
+                               void* workspace, int64_t workspace_bytes, void* stream) {
   if (M < 0 || N < 0 || K <= 0 || K % kMxBlock) {
     set_error("mxfp4_mm: bad sizes M=%lld N=%lld K=%lld (K in whole blocks of 32)", (long long)M,
               (long long)N, (long long)K);
@@ -80,9 +101,22 @@ extern "C" int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int
   const MxMM p{a, b, scale_a, scale_b, lda, ldb, ldsa, ldsb, bias, out, ldc, M, N, K,
                bias ? bias_dtype : I8L_DTYPE_NONE, out_dtype};
   const hipStream_t st = (hipStream_t)stream;
-  const hipError_t e = p.M > 128 && mx_phased_ok(p) ? launch_mx_phased(p, st)
-                       : mx_ring_ok(p)              ? launch_mx_ring(p, st)
-                       : mx_decode_ok(p)            ? launch_mx_decode(p, st)
-                                                    : launch_mx_any(p, st);
+  // a workspace is taken whole or not at all
+  const int64_t need = i8l_mxfp4_mm_workspace_bytes(M, N, K);
+  const bool split = need > 0 && workspace && workspace_bytes >= need && aligned16(workspace);
+  const hipError_t e = mx_phased_ok(p) && (many_tokens(M, N, K, split) || !mx_ring_ok(p))
+                           ? launch_mx_phased(p, workspace, split ? kMostWorkspace : 0, st)
+                       : mx_ring_ok(p)   ? launch_mx_ring(p, st)
+                       : mx_decode_ok(p) ? launch_mx_decode(p, st)
+                                         : launch_mx_any(p, st);
   return hip_status(e, "mxfp4_mm launch");
+}
+
+extern "C" int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
+                            const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b,
+                            int64_t ldsb, const void* bias, int32_t bias_dtype, void* out,
+                            int64_t ldc, int32_t out_dtype, int64_t M, int64_t N, int64_t K,
+                            void* stream) {
+  return i8l_mxfp4_mm_ws(a, lda, b, ldb, scale_a, ldsa, scale_b, ldsb, bias, bias_dtype, out, ldc,
+                         out_dtype, M, N, K, nullptr, 0, stream);
 }

@@ -55,8 +55,11 @@ __device__ __forceinline__ void bias4(const MxMM& p, int64_t n, float (&b)[4]) {
   }
 }
 
-template <int QA, int QB0, int QB1, int OD, bool BIAS>
-__global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int tiles) {
+// SPLIT: K in `splits` parts, each a tile's work of its own, whose fp32 sums go to a plane of M x N
+// of p.out each (OD fp32, no bias).
+template <int QA, int QB0, int QB1, int OD, bool BIAS, bool SPLIT>
+__global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int tiles, int splits) {
+  static_assert(!SPLIT || (OD == I8L_F32 && !BIAS), "parts are raw sums");
   constexpr int W = 4, WN = 2, BK = 128;
   constexpr int QB[2] = {QB0, QB1};
   constexpr int QN = QB0 + QB1;                      // column fragments of a wave
@@ -80,7 +83,8 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int num_pid_m = (M + BM - 1) / BM, num_pid_n = (N + BN - 1) / BN;
-  const int KT = (int)(p.K / (2 * BK));
+  const int pairs = (int)(p.K / (4 * BK));   // K steps come in pairs
+  const int work = SPLIT ? tiles * splits : tiles;
 
   // Copies of codes: copy j of a half writes LDS rows [RPC x, RPC x + RPC), x = W j + wave; lane l
   // writes slot l % CPR of row l / CPR.  Half row r lies in wave block r / R of that half.
@@ -110,7 +114,17 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
   const uint8_t *pA, *pB;      // the K position being requested, in the tile being requested
   const uint8_t *psA, *psB;    // the batch of scales being requested
   int sreq = 0;                // its buffer (bytes from SC0)
-  auto tile_at = [&](int tile, int64_t& mt, int64_t& nt) {
+  // the tile, the first K step and the number of steps of a piece of work
+  auto work_at = [&](int piece, int64_t& mt, int64_t& nt, int& k0, int& kt) {
+    const int tile = SPLIT ? piece % tiles : piece, part = SPLIT ? piece / tiles : 0;
+    if constexpr (SPLIT) {
+      const int most = pairs / splits, more = pairs % splits;
+      k0 = 2 * (part * most + min(part, more));
+      kt = 2 * (most + (part < more));
+    } else {
+      k0 = 0;
+      kt = 2 * pairs;
+    }
     int pid_m, pid_n;
     staged_tile(tiles % 8 == 0 ? tile : xcd_order(tile, tiles), tiles, num_pid_m, num_pid_n, group_m,
                 pid_m, pid_n);
@@ -120,11 +134,11 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
   };
   // copy j of the batch: rows [64 x, 64 x + 64) of the tile's A rows and then B rows
   auto scale_copy = [&](int j) { return min(W * j + wave, SC - 1); };
-  auto request_from = [&](int64_t mt, int64_t nt) {
-    pA = p.a + mt * p.lda;
-    pB = p.b + nt * p.ldb;
-    psA = p.sa + mt * p.ldsa;
-    psB = p.sb + nt * p.ldsb;
+  auto request_from = [&](int64_t mt, int64_t nt, int k0) {
+    pA = p.a + mt * p.lda + (int64_t)k0 * BK;
+    pB = p.b + nt * p.ldb + (int64_t)k0 * BK;
+    psA = p.sa + mt * p.ldsa + k0 * 8;
+    psB = p.sb + nt * p.ldsb + k0 * 8;
     const int last = M - 1 - (int)mt;   // token rows past M copy the last row, never stored
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -277,10 +291,10 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
     pB += BK;
   };
 
-  int tile = blockIdx.x;
+  int piece = blockIdx.x, k0, KT;
   int64_t m0, n0;
-  tile_at(tile, m0, n0);
-  request_from(m0, n0);
+  work_at(piece, m0, n0, k0, KT);
+  request_from(m0, n0, k0);
   copyS();
   request_step(P0{});
   request_step(P1{});
@@ -298,18 +312,29 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
     if (!landed) wait_vmcnt<3 * JA + JB[0] + JB[1]>();
     lds_barrier();
 
-    const int next = tile + gridDim.x;   // past the last tile: its own start again, not used
+    const int next = piece + gridDim.x;   // past the last piece: its own start again, not used
     int64_t m1 = m0, n1 = n0;
-    if (next < tiles) tile_at(next, m1, n1);
+    int k1 = k0, KT1 = KT;
+    if (next < work) work_at(next, m1, n1, k1, KT1);
     step(P0{}, std::false_type{}, std::integral_constant<int, 4>{}, landed);
     step(P1{}, std::false_type{}, std::integral_constant<int, 1>{}, landed);
     for (int t = 2; t + 2 < KT; t += 2) {
       step(P0{}, std::false_type{}, P0{}, false);
       step(P1{}, std::false_type{}, P0{}, false);
     }
-    request_from(m1, n1);
+    request_from(m1, n1, k1);
     step(P0{}, std::false_type{}, P0{}, false);
     step(P1{}, std::true_type{}, P0{}, false);
+    // the sums stay in AGPRs up to here: with the epilogue's use of them in sight, the compiler
+    // moves the last steps' into VGPRs and spills 120 others (256 x 256)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+        for (int i = 0; i < QA; ++i)
+#pragma unroll
+          for (int j = 0; j < QB[hb]; ++j) asm volatile("" : "+a"(acc[h][hb][i][j]));
 
     // ---- epilogue: the bias in fp32, one cast.  Each wave takes 32 tokens x 64 columns (16-bit
     // outputs; 32 columns of 4-byte ones) at a time through its 4 KiB: rows of 128 bytes, chunk c
@@ -321,6 +346,7 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
     const int erow = ln & 31, ehalf = ln >> 5, srow = ln >> 3, sch = ln & 7;
     const int64_t nw = n0 + wn * 32 * QN, mw = m0 + wm * 64 * QA;
     int8_t* stg = lds + STG + wave * 4096;
+    float* plane = SPLIT ? (float*)p.out + (int64_t)(piece / tiles) * M * p.ldc : (float*)p.out;
 #pragma unroll
     for (int g = 0; g < (QN + 1) / 2; ++g) {   // fragments 2g and 2g+1 of the wave's columns
       const int nf = QN % 2 == 1 && g == QN / 2 ? 1 : 2;   // (an odd last fragment stands alone)
@@ -362,9 +388,11 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
               for (int y = 0; y < 4; ++y) {
                 const int row = 8 * y + srow;
                 const v4i v = *(const v4i*)(stg + row * 128 + ((sch ^ srow) * 16));
-                if (mb + row < M)
-                  __builtin_nontemporal_store(
-                      v, (v4i*)((int32_t*)p.out + (mb + row) * p.ldc + nw + 32 * x + 4 * sch));
+                v4i* at = (v4i*)(plane + (mb + row) * p.ldc + nw + 32 * x + 4 * sch);
+                if (mb + row < M) {
+                  if constexpr (SPLIT) *at = v;   // read again at once
+                  else __builtin_nontemporal_store(v, at);
+                }
               }
             }
           } else {
@@ -390,40 +418,83 @@ __global__ void __launch_bounds__(256) mxfp4_phased(MxMM p, int group_m, int til
         }
       asm volatile("" ::: "memory");   // the next 64 columns' operands load after these
     }
-    if (next >= tiles) break;
-    tile = next;
+    if (next >= work) break;
+    piece = next;
     m0 = m1;
     n0 = n1;
+    k0 = k1;
+    KT = KT1;
     landed = true;
   }
 }
 
+// The sum of the parts' planes in order, the bias and one rounding; a thread four columns.
+template <int OD>
+__global__ void __launch_bounds__(256) mxfp4_sum_parts(MxMM p, const float* __restrict__ parts,
+                                                       int splits) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, plane = p.M * p.N;
+  if (i >= plane) return;
+  v4f v = *(const v4f*)(parts + i);
+  for (int z = 1; z < splits; ++z) v += *(const v4f*)(parts + z * plane + i);
+  const int64_t m = i / p.N, n = i % p.N;
+  if (p.bias) {
+    float b[4];
+    bias4(p, n, b);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] += b[r];
+  }
+  if constexpr (OD == I8L_F32) {
+    *(v4f*)((float*)p.out + m * p.ldc + n) = v;
+  } else {
+    *(uint2*)((uint16_t*)p.out + m * p.ldc + n) =
+        make_uint2(f32x2_to_act2<OD>(v[0], v[1]), f32x2_to_act2<OD>(v[2], v[3]));
+  }
+}
+
 // ------------------------------------------------------------------ host side
+// The tiles, and what a piece of work on one was measured to take (us): a K step with the card
+// nearly idle and with a piece on every CU (the clock falls as the card fills), and the rest.
 struct PhasedTile {
   int bm, bn;
+  float step_idle, step_full, rest;
 };
-constexpr PhasedTile kTiles[] = {{256, 256}, {256, 192}, {256, 128}, {128, 256}, {128, 192}, {128, 128}};
+constexpr PhasedTile kTiles[] = {{256, 256, 1.04f, 1.72f, 4.5f}, {256, 192, 0.94f, 1.35f, 4.0f},
+                                 {256, 128, 0.75f, 1.05f, 2.8f}, {128, 256, 0.87f, 1.05f, 2.8f},
+                                 {128, 192, 0.78f, 0.88f, 2.5f}, {128, 128, 0.66f, 0.72f, 1.2f}};
 
-template <int QA, int QB0, int QB1, int OD, bool BIAS>
-hipError_t launch_phased_k(const MxMM& p, int group_m, hipStream_t st) {
-  auto kern = mxfp4_phased<QA, QB0, QB1, OD, BIAS>;
+template <int QA, int QB0, int QB1, int OD, bool BIAS, bool SPLIT>
+hipError_t launch_phased_k(const MxMM& p, int splits, hipStream_t st) {
+  auto kern = mxfp4_phased<QA, QB0, QB1, OD, BIAS, SPLIT>;
   constexpr int BM = 128 * QA, BN = 64 * (QB0 + QB1);
   constexpr size_t shm = 2 * (size_t)(BM + BN) * (128 + 16) + 4 * 4096;
   static_assert(shm <= kMaxLds, "two buffers, two batches of scales and the staging fit the LDS");
   static std::atomic<uint64_t> lds_done{0};
   lds_opt_in((const void*)kern, shm, lds_done);
   const int tiles = (int)((p.M + BM - 1) / BM * ((p.N + BN - 1) / BN));
-  const int grid = std::min(tiles, cu_count() * (int)(kMaxLds / shm));
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), shm, st, p, group_m, tiles);
+  const int grid = std::min(tiles * splits, cu_count() * (int)(kMaxLds / shm));
+  // 8 rows of tiles walked together (4096 x 28672: 2 rows 226 us, 4 222, 8 221, 16 223)
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), shm, st, p, 8, tiles, splits);
   return hipGetLastError();
 }
 
 template <int QA, int QB0, int QB1>
-hipError_t launch_phased_t(const MxMM& p, int gm, hipStream_t st) {
+hipError_t launch_phased_t(const MxMM& p, int splits, float* parts, hipStream_t st) {
+  if (splits > 1) {
+    MxMM q = p;
+    q.out = parts, q.ldc = p.N, q.out_dtype = I8L_F32, q.bias = nullptr;
+    const hipError_t e = launch_phased_k<QA, QB0, QB1, I8L_F32, false, true>(q, splits, st);
+    if (e) return e;
+    const dim3 grid((unsigned)((p.M * p.N + 1023) / 1024));
+    auto sum = p.out_dtype == I8L_BF16  ? mxfp4_sum_parts<I8L_BF16>
+               : p.out_dtype == I8L_F16 ? mxfp4_sum_parts<I8L_F16>
+                                        : mxfp4_sum_parts<I8L_F32>;
+    hipLaunchKernelGGL(sum, grid, dim3(256), 0, st, p, parts, splits);
+    return hipGetLastError();
+  }
   auto go = [&](auto odc) {
     constexpr int OD = decltype(odc)::value;
-    return p.bias ? launch_phased_k<QA, QB0, QB1, OD, true>(p, gm, st)
-                  : launch_phased_k<QA, QB0, QB1, OD, false>(p, gm, st);
+    return p.bias ? launch_phased_k<QA, QB0, QB1, OD, true, false>(p, 1, st)
+                  : launch_phased_k<QA, QB0, QB1, OD, false, false>(p, 1, st);
   };
   switch (p.out_dtype) {
     case I8L_BF16: return go(std::integral_constant<int, I8L_BF16>{});
@@ -441,22 +512,52 @@ bool mx_phased_ok(const MxMM& p) {
          p.ldsb % 16 == 0 && p.ldc * es % 16 == 0 && p.K % 512 == 0 && p.K >= 1024 && p.N % 8 == 0 &&
          p.N >= 128 && p.lda <= 1 << 22 && p.ldb <= 1 << 22 && p.ldsa <= 1 << 22 &&
          p.ldsb <= 1 << 22 && p.M < (int64_t)1 << 30 && p.N < (int64_t)1 << 30 &&
-         (p.M + 127) / 128 * ((p.N + 127) / 128) < (int64_t)1 << 30;
+         (p.M + 127) / 128 * ((p.N + 127) / 128) < (int64_t)1 << 26;
 }
 
-hipError_t launch_mx_phased_tile(int t, int gm, const MxMM& p, hipStream_t st) {
+hipError_t launch_mx_phased_tile(int t, int splits, float* parts, const MxMM& p, hipStream_t st) {
   switch (t) {
-    case 0: return launch_phased_t<2, 2, 2>(p, gm, st);
-    case 1: return launch_phased_t<2, 2, 1>(p, gm, st);
-    case 2: return launch_phased_t<2, 1, 1>(p, gm, st);
-    case 3: return launch_phased_t<1, 2, 2>(p, gm, st);
-    case 4: return launch_phased_t<1, 2, 1>(p, gm, st);
+    case 0: return launch_phased_t<2, 2, 2>(p, splits, parts, st);
+    case 1: return launch_phased_t<2, 2, 1>(p, splits, parts, st);
+    case 2: return launch_phased_t<2, 1, 1>(p, splits, parts, st);
+    case 3: return launch_phased_t<1, 2, 2>(p, splits, parts, st);
+    case 4: return launch_phased_t<1, 2, 1>(p, splits, parts, st);
   }
-  return launch_phased_t<1, 1, 1>(p, gm, st);
+  return launch_phased_t<1, 1, 1>(p, splits, parts, st);
 }
 
-hipError_t launch_mx_phased(const MxMM& p, hipStream_t st) {
-  return launch_mx_phased_tile(p.N >= 256 ? 0 : 5, 4, p, st);
+// The tile and the parts of K with the least modelled time: rounds of a piece on every CU, each the
+// piece's steps and rest, and for parts the sum's launch and traffic (S planes written and read at
+// 4.4 TB/s).  Measured against it (cold weights, us; unsplit / split): 14336 -> 4096 at 128 tokens
+// 30 / 17.8 in 7 parts, at 256 33 / 22.7 in 4, at 512 41.8 / 31.7 in 2; 2048 -> 4096 at 512 6.9 / 18.4.
+MxPhasedPlan mx_phased_plan(int64_t M, int64_t N, int64_t K, int64_t workspace) {
+  MxPhasedPlan best{-1, 1};
+  double least = 0;
+  const int64_t pairs = K / 512;
+  const int cus = 256;
+  for (int t = 0; t < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++t) {
+    const PhasedTile& tile = kTiles[t];
+    if (N < tile.bn) continue;
+    const int64_t tiles = (M + tile.bm - 1) / tile.bm * ((N + tile.bn - 1) / tile.bn);
+    for (int64_t s = 1; s <= kMaxParts && 2 * s <= pairs; ++s) {
+      if (s > 1 && (s * M * N * 4 > workspace || tiles * s > cus)) break;
+      const double steps = 2.0 * ((pairs + s - 1) / s);
+      const int64_t work = tiles * s, rest = work % cus;
+      const double load = (double)rest / cus;
+      double us = (double)(work / cus) * (steps * tile.step_full + tile.rest);
+      if (rest)
+        us += steps * (tile.step_idle + (tile.step_full - tile.step_idle) * load) + tile.rest;
+      if (s > 1) us += 2.5 + 8.0 * s * M * N / 4.4e6;
+      if (best.tile < 0 || us < least) best = {t, (int)s}, least = us;
+    }
+  }
+  return best;
+}
+
+hipError_t launch_mx_phased(const MxMM& p, void* workspace, int64_t bytes, hipStream_t st) {
+  const MxPhasedPlan plan =
+      mx_phased_plan(p.M, p.N, p.K, workspace && aligned16(workspace) ? bytes : 0);
+  return launch_mx_phased_tile(plan.tile, plan.splits, (float*)workspace, p, st);
 }
 
 }  // namespace i8l

@@ -367,12 +367,16 @@ py::object mxfp4_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& 
     bias_ptr = bt.data_ptr();
   }
   at::Tensor out = empty_like_on(a, {M, N}, out_dtype);
+  const int64_t ws_bytes = i8l_mxfp4_mm_workspace_bytes(M, N, K);
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = empty_like_on(a, {ws_bytes}, at::kByte);
   const c10::DeviceGuard guard(dev);
-  const int st = i8l_mxfp4_mm((const uint8_t*)a.data_ptr(), row_stride(a),
+  const int st = i8l_mxfp4_mm_ws((const uint8_t*)a.data_ptr(), row_stride(a),
                               (const uint8_t*)b.data_ptr(), N > 1 ? b.stride(1) : K / 2,
                               (const uint8_t*)sa.data_ptr(), row_stride(sa),
                               (const uint8_t*)sb.data_ptr(), row_stride(sb), bias_ptr, bias_code,
-                              out.data_ptr(), N, out_code, M, N, K, stream_of(a));
+                              out.data_ptr(), N, out_code, M, N, K,
+                              ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(a));
   if (st != I8L_OK) return py::none();
   ++g_launches;
   return py::cast(out);

@@ -17,7 +17,8 @@ for each call.  Both operands' scales enter the matrix instructions themselves
 (v_mfma_scale_f32_*_f8f6f4), which accumulate in fp32.  A linear reads 17/32 of a byte a weight,
 0.53 of the int8 path's, and the instruction does twice the int8 one's operations.
 
-Launches go on the caller's current stream and allocate nothing but the outputs.
+Launches go on the caller's current stream and allocate nothing but the outputs, and for some
+products of 73 to 512 tokens and a long K the partial sums of its parts.
 """
 
 from __future__ import annotations
@@ -221,11 +222,15 @@ def mxfp4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_
     a_q, w_q, scale_a, scale_b = (t if t.shape[0] <= 1 or t.stride(0) >= t.shape[1] else t.contiguous()
                                   for t in (a_q, w_q, scale_a, scale_b))
     out = torch.empty((m, n), dtype=out_dtype, device=a_q.device)
+    # the fp32 sums of a split of K, from the caching allocator (the graph's pool under capture)
+    need = _lib.lib().i8l_mxfp4_mm_workspace_bytes(m, n, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=a_q.device) if need else None
     with torch.cuda.device(a_q.device):
-        status = _lib.lib().i8l_mxfp4_mm(
+        status = _lib.lib().i8l_mxfp4_mm_ws(
             a_q.data_ptr(), _ld(a_q), w_q.data_ptr(), _ld(w_q), scale_a.data_ptr(), _ld(scale_a),
             scale_b.data_ptr(), _ld(scale_b), bias.data_ptr() if bias is not None else None,
-            bias_code, out.data_ptr(), n, out_code, m, n, k, _lib.stream_of(a_q))
+            bias_code, out.data_ptr(), n, out_code, m, n, k, ws.data_ptr() if need else None, need,
+            _lib.stream_of(a_q))
     _lib.check(status, NotSupported)
     return out
 

@@ -263,7 +263,9 @@ def test_mm_exact(m, n, k):
 
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 2048), (5, 2048, 6144), (24, 12288, 2048), (75, 4096, 7168),
                                    (513, 1024, 2048), (777, 1536, 4096), (1000, 520, 1536),
-                                   (2049, 256, 1024)])
+                                   (2049, 256, 1024), (100, 1024, 14336), (300, 512, 8192),
+                                   (129, 2048, 6144), (640, 392, 6144), (40, 28672, 1024),
+                                   (90, 12288, 1536)])
 def test_mm_exact_served_sizes(m, n, k):
     _check_exact(m, n, k)
 
@@ -325,6 +327,35 @@ def test_mm_nan_scales_reach_their_rows_and_columns_only(m, n, k):
     assert torch.equal(torch.isnan(out), bad)
     want = torch.from_numpy(mx.mm(a, sa, w, sw)[0]).float()
     assert torch.equal(out[~bad], want[~bad])
+
+
+@pytest.mark.parametrize("m,n,k", [(100, 1024, 14336), (200, 136, 6144)])
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_mm_with_and_without_a_workspace(m, n, k, dt):
+    """The split of K, with its workspace NULL, too small, misaligned or given; nothing is written
+    past what it needs."""
+    a, sa, ad, sad = _operand(m, k, 1)
+    w, sw, wd, swd = _operand(n, k, 2)
+    bias = torch.arange(n).to(DT[dt]).cuda()
+    # (the bias as its type holds it: bf16 has no 257)
+    want, terms = mx.mm(a, sa, w, sw, bias.double().cpu().numpy())
+    assert terms.max() + n < 2.0 ** (int(sa.min()) + int(sw.min()) - 256 + 23)
+    L = _lib.lib()
+    need = L.i8l_mxfp4_mm_workspace_bytes(m, n, k)
+    assert need >= 2 * m * n * 4 and need % (m * n * 4) == 0
+    ws = torch.full((need + 64,), 0xA5, dtype=torch.uint8, device="cuda")
+    for ptr, size in ((None, need), (ws.data_ptr(), need - 1), (ws.data_ptr() + 4, need + 32),
+                      (ws.data_ptr(), need)):
+        out = torch.full((m + 1, n), 7.0, dtype=DT[dt], device="cuda")
+        st = L.i8l_mxfp4_mm_ws(ad.data_ptr(), k // 2, wd.data_ptr(), k // 2, sad.data_ptr(), k // 32,
+                               swd.data_ptr(), k // 32, bias.data_ptr(), _lib.DTYPE_CODE[DT[dt]],
+                               out.data_ptr(), n, _lib.DTYPE_CODE[DT[dt]], m, n, k, ptr, size,
+                               _lib.stream_of(ad))
+        assert st == _lib.OK
+        used = ptr == ws.data_ptr() and size == need
+        assert bool((ws[:need] == 0xA5).all()) != used and (ws[need:] == 0xA5).all()
+        assert torch.equal(out[:m].cpu(), torch.from_numpy(want).float().to(DT[dt]))
+        assert (out[m] == 7).all()
 
 
 def test_mm_of_nothing_and_shared_rows():
@@ -395,6 +426,31 @@ def test_calls_in_a_graph_replay_as_eager_ones(m):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(r, want[0]) and torch.equal(out, want[1])
+
+
+def test_a_split_of_k_in_a_graph():
+    """Two graphs of one split product each, replayed on two streams at once: each has its own sums."""
+    w = mxfp4.mxfp4_quant(_x((512, 8192), 1, torch.bfloat16, 0.5).cuda())
+    assert _lib.lib().i8l_mxfp4_mm_workspace_bytes(200, 512, 8192) > 0
+    cases = []
+    for i in range(2):
+        x = mxfp4.mxfp4_quant(_x((200, 8192), 5 + i, torch.bfloat16, 0.5).cuda())
+        call = lambda x=x: mxfp4.mxfp4_mm(x[0], w[0].t(), x[1], w[1], torch.float32)   # noqa: E731
+        want = call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        cases.append((graph, out, want, torch.cuda.Stream()))
+    for _ in range(5):
+        for graph, out, _, stream in cases:
+            out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for graph, _, _, stream in cases:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for _, out, want, _ in cases)
 
 
 def test_calls_on_another_stream():
