@@ -24,12 +24,14 @@ namespace {
 template <int J>
 __device__ __forceinline__ void store_scales(const uint32_t (&code)[J], uint8_t* srow, int64_t e0,
                                              int64_t n, int lane) {
-  const int j = lane & 3;
-  uint32_t c = code[0];
+  // the bytes of one word, picked by a shift (a choice among the array's elements goes through LDS,
+  // addressed by the block size, which is read from the dispatch packet in host memory: +13 us)
+  uint32_t w = code[0];
 #pragma unroll
-  for (int i = 1; i < J; ++i) c = j == i ? code[i] : c;
+  for (int i = 1; i < J; ++i) w |= code[i] << (8 * i);
+  const int j = lane & 3;
   const int64_t e = e0 + (int64_t)(j * 64 + (lane & 60)) * 8;
-  if (j < J && e < n) srow[e / kMxBlock] = (uint8_t)c;
+  if (j < J && e < n) srow[e / kMxBlock] = (uint8_t)(w >> (8 * j));
 }
 
 // One word of codes to q (element e0 of a row of n); VEC: q is 4-byte aligned.

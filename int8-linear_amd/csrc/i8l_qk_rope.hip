@@ -12,7 +12,10 @@
 // values R/2 apart, so both members of every pair of either kind are its own and nothing but the sum
 // of squares crosses lanes (L lanes a head, a power of two: DPP steps), each load is 16 bytes, and a
 // head that is written over its own input is read whole by the lanes that write it.  A wave takes
-// 64/L heads at a time of one token, whose cos, sin and the two weights stay in its registers.
+// 64/L heads at a time of one token, whose cos, sin and the two weights stay in its registers; they
+// are loaded 16 bytes at a time, with no choice of type inside (a value at a time, a token of 16 + 8
+// heads takes 6.2 us; so 3.3).  4096 tokens of 32 + 8 heads of 128: 19.7 us, 4.3 TB/s; a copy of as
+// many bytes takes 18.
 #include <algorithm>
 
 #include "i8l_common.h"
@@ -81,14 +84,47 @@ __device__ __forceinline__ void store_run(uint16_t* p, const float (&v)[V]) {
   else *(uint2*)p = make_uint2(w[0], w[1]);
 }
 
+// N consecutive values of a table or weight as floats, by one load of 16 bytes or two; F32: of fp32,
+// else of the 16-bit dtype dt.
+template <int N, bool F32>
+__device__ __forceinline__ void load_floats(const void* p, int dt, int64_t at, float (&o)[N]) {
+  if constexpr (F32) {
+    const float* f = (const float*)p + at;
+    if constexpr (N == 2) {
+      const float2 v = *(const float2*)f;
+      o[0] = v.x, o[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 v = *(const float4*)(f + i);
+        o[i] = v.x, o[i + 1] = v.y, o[i + 2] = v.z, o[i + 3] = v.w;
+      }
+    }
+  } else {
+    const uint16_t* h = (const uint16_t*)p + at;
+    uint32_t w[N / 2];
+    if constexpr (N == 2) {
+      w[0] = *(const uint32_t*)h;
+    } else {
+      const Run<N> r = load_run<N>(h);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) w[i] = r.w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = act_to_f32(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu, dt);
+  }
+}
+
 // L lanes a head: the first R / 2V own the rotated runs [V j, V j + V) and R/2 further, the next
-// ones two runs of the rest, the others none.
-template <int DT, int V, bool INTER>
+// ones two runs of the rest, the others none.  C32: the table is fp32; W32: the weights are (or there
+// is none).
+template <int DT, int V, bool INTER, bool C32, bool W32>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs a, int L, int logL) {
   const uint32_t wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t t = wave / (uint32_t)a.parts;
   if (t >= a.T) return;
   const int part = wave % (uint32_t)a.parts;
+  const int64_t row = table_row(a, t);
   const int lane = threadIdx.x & 63, j = lane & (L - 1), sub = lane >> logL;
   const int per = 64 >> logL, heads = a.hq + a.hk, groups = (heads + per - 1) / per;
   const int rl = a.R / (2 * V);
@@ -97,47 +133,63 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs a, int L, int 
   const int d1 = turned ? d0 + a.R / 2 : d0 + V;
   const bool in0 = d0 < a.D, in1 = d1 < a.D;
 
+  const uint16_t *q = (const uint16_t*)a.q + t * a.q_ts, *k = (const uint16_t*)a.k + t * a.k_ts;
+  uint16_t *qo = (uint16_t*)a.qo + t * a.qo_ts, *ko = (uint16_t*)a.ko + t * a.ko_ts;
   struct Head {
-    const uint16_t* in;
-    uint16_t* out;
+    int i;        // among the queries, or the keys
     bool q, on;
   };
   auto head_at = [&](int g) {
     Head h;
-    int i = g * per + sub;
-    h.on = g < groups && i < heads;
-    h.q = i < a.hq;
-    if (!h.q) i -= a.hq;
-    h.in = (const uint16_t*)(h.q ? a.q : a.k) + t * (h.q ? a.q_ts : a.k_ts) +
-           (int64_t)i * (h.q ? a.q_hs : a.k_hs);
-    h.out = (uint16_t*)(h.q ? a.qo : a.ko) + t * (h.q ? a.qo_ts : a.ko_ts) +
-            (int64_t)i * (h.q ? a.qo_hs : a.ko_hs);
+    h.i = g * per + sub;
+    h.on = g < groups && h.i < heads;
+    h.q = h.i < a.hq;
+    if (!h.q) h.i -= a.hq;
     return h;
   };
   auto load = [&](const Head& h, Run<V>(&r)[2]) {
+    const uint16_t* p = (h.q ? q : k) + h.i * (int)(h.q ? a.q_hs : a.k_hs);
     r[0] = Run<V>{}, r[1] = Run<V>{};
-    if (h.on && in0) r[0] = load_run<V>(h.in + d0);
-    if (h.on && in1) r[1] = load_run<V>(h.in + d1);
+    if (h.on && in0) r[0] = load_run<V>(p + d0);
+    if (h.on && in1) r[1] = load_run<V>(p + d1);
   };
 
   Head h = head_at(part);
   Run<V> raw[2];
   load(h, raw);
-  // the token's angles (cs[0] for run 0's first value on; interleaved runs have V/2 each) and weights
-  const int64_t row = table_row(a, t);
-  float c[V], s[V], wq[2][V], wk[2][V];
+  float wq[2][V], wk[2][V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    c[i] = 1.0f, s[i] = 0.0f;
-    if (turned) {
-      const int at = INTER ? (i < V / 2 ? d0 / 2 + i : d1 / 2 + i - V / 2) : d0 + i;
-      c[i] = row >= 0 ? load_f(a.cs, a.cs_dtype, row * a.R + at) : __builtin_nanf("");
-      s[i] = row >= 0 ? load_f(a.cs, a.cs_dtype, row * a.R + a.R / 2 + at) : __builtin_nanf("");
+  for (int i = 0; i < V; ++i) wq[0][i] = wq[1][i] = wk[0][i] = wk[1][i] = 1.0f;
+  if (a.qw) {
+    if (in0) load_floats<V, W32>(a.qw, a.w_dtype, d0, wq[0]);
+    if (in1) load_floats<V, W32>(a.qw, a.w_dtype, d1, wq[1]);
+  }
+  if (a.kw) {
+    if (in0) load_floats<V, W32>(a.kw, a.w_dtype, d0, wk[0]);
+    if (in1) load_floats<V, W32>(a.kw, a.w_dtype, d1, wk[1]);
+  }
+  // the token's angles; the two runs have the same ones, or V/2 each when interleaved
+  float c[V], s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) c[i] = 1.0f, s[i] = 0.0f;
+  if (turned) {
+    const int64_t at = row * a.R;
+    if (row < 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) c[i] = s[i] = __builtin_nanf("");
+    } else if constexpr (INTER) {
+      float c0[V / 2], c1[V / 2], s0[V / 2], s1[V / 2];
+      load_floats<V / 2, C32>(a.cs, a.cs_dtype, at + d0 / 2, c0);
+      load_floats<V / 2, C32>(a.cs, a.cs_dtype, at + d1 / 2, c1);
+      load_floats<V / 2, C32>(a.cs, a.cs_dtype, at + a.R / 2 + d0 / 2, s0);
+      load_floats<V / 2, C32>(a.cs, a.cs_dtype, at + a.R / 2 + d1 / 2, s1);
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i)
+        c[i] = c0[i], c[V / 2 + i] = c1[i], s[i] = s0[i], s[V / 2 + i] = s1[i];
+    } else {
+      load_floats<V, C32>(a.cs, a.cs_dtype, at + d0, c);
+      load_floats<V, C32>(a.cs, a.cs_dtype, at + a.R / 2 + d0, s);
     }
-    wq[0][i] = a.qw && in0 ? load_f(a.qw, a.w_dtype, d0 + i) : 1.0f;
-    wq[1][i] = a.qw && in1 ? load_f(a.qw, a.w_dtype, d1 + i) : 1.0f;
-    wk[0][i] = a.kw && in0 ? load_f(a.kw, a.w_dtype, d0 + i) : 1.0f;
-    wk[1][i] = a.kw && in1 ? load_f(a.kw, a.w_dtype, d1 + i) : 1.0f;
   }
   for (int g = part; g < groups; g += a.parts) {
     const Head next = head_at(g + a.parts);
@@ -175,8 +227,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs a, int L, int 
         x[1][i] = __builtin_fmaf(v, c[i], u * s[i]);
       }
     }
-    if (h.on && in0) store_run<V, DT>(h.out + d0, x[0]);
-    if (h.on && in1) store_run<V, DT>(h.out + d1, x[1]);
+    uint16_t* p = (h.q ? qo : ko) + h.i * (int)(h.q ? a.qo_hs : a.ko_hs);
+    if (h.on && in0) store_run<V, DT>(p + d0, x[0]);
+    if (h.on && in1) store_run<V, DT>(p + d1, x[1]);
     h = next;
     raw[0] = ahead[0], raw[1] = ahead[1];
   }
@@ -220,8 +273,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(QkArgs a, int int
   for (int d = a.R + lane; d < a.D; d += 64) out[d] = f32_to_act<DT>(normed(d));
 }
 
-// Waves that fill the card: a token's heads are spread over more waves until there are this many
-// (256 CUs, 4 SIMDs, 4 waves a SIMD).
+// Waves that fill the card: a token's heads are spread over more waves until there are this many (256
+// CUs, 4 SIMDs, 4 waves a SIMD).  More repeat the token's angles and weights: 2048 tokens of 16 + 8
+// heads 8.7 us, at four times the waves 10.1; 4096 of 32 + 8 19.7, at twice 20.3, at four times 23.8.
 constexpr int64_t kQkWaves = 4096;
 
 template <int DT, int V, bool INTER>
@@ -230,8 +284,12 @@ void launch_qk(QkArgs a, int L, hipStream_t st) {
   while ((1 << logL) < L) ++logL;
   const int per = 64 / L, groups = (a.hq + a.hk + per - 1) / per;
   a.parts = (int)std::min<int64_t>(groups, std::max<int64_t>(1, (kQkWaves + a.T - 1) / a.T));
-  hipLaunchKernelGGL((qk_norm_rope_kernel<DT, V, INTER>),
-                     dim3((unsigned)((a.T * a.parts + 3) / 4)), dim3(256), 0, st, a, L, logL);
+  const bool w32 = a.w_dtype == I8L_F32 || !(a.qw || a.kw);
+  auto kern = a.cs_dtype == I8L_F32 ? (w32 ? qk_norm_rope_kernel<DT, V, INTER, true, true>
+                                           : qk_norm_rope_kernel<DT, V, INTER, true, false>)
+                                    : (w32 ? qk_norm_rope_kernel<DT, V, INTER, false, true>
+                                           : qk_norm_rope_kernel<DT, V, INTER, false, false>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((a.T * a.parts + 3) / 4)), dim3(256), 0, st, a, L, logL);
 }
 
 }  // namespace
@@ -282,11 +340,14 @@ extern "C" int i8l_qk_norm_rope(const void* q, int64_t q_ts, int64_t q_hs, const
   auto runs = [&](int V) {
     const int64_t b = 2 * V;
     auto at = [&](const void* p, int64_t ts, int64_t hs, int64_t n) {
-      return !n || ((uintptr_t)p % b == 0 && ts % V == 0 && hs % V == 0);
+      return !n || ((uintptr_t)p % b == 0 && ts % V == 0 && hs % V == 0 && hs >= 0 &&
+                    (n - 1) * hs + D < INT32_MAX);
     };
+    auto whole = [&](const void* p) { return (uintptr_t)p % 16 == 0; };
     const int64_t lanes = R / (2 * V) + (D - R + 2 * V - 1) / (2 * V);
     return R % (2 * V) == 0 && D % V == 0 && lanes <= 64 && at(q, q_ts, q_hs, Hq) &&
-           at(q_out, qo_ts, qo_hs, Hq) && at(k, k_ts, k_hs, Hk) && at(k_out, ko_ts, ko_hs, Hk);
+           at(q_out, qo_ts, qo_hs, Hq) && at(k, k_ts, k_hs, Hk) && at(k_out, ko_ts, ko_hs, Hk) &&
+           whole(cos_sin) && whole(q_weight) && whole(k_weight);
   };
   const int V = runs(8) ? 8 : runs(4) ? 4 : 0;
   const hipStream_t st = (hipStream_t)stream;
