@@ -64,9 +64,11 @@ bool phased_sizes(int64_t M, int64_t N, int64_t K) {
 using namespace i8l;
 
 extern "C" int64_t i8l_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (!phased_sizes(M, N, K) || M > 4096 || N > INT32_MAX || K > INT32_MAX) return 0;
+  if (!phased_sizes(M, N, K) || M > 4096 || N > INT32_MAX || K > INT32_MAX ||
+      !many_tokens(M, N, K, true))
+    return 0;
   const int splits = mx_phased_plan(M, N, K, kMostWorkspace).splits;
-  return splits > 1 && many_tokens(M, N, K, true) ? splits * M * N * 4 : 0;
+  return splits > 1 ? splits * M * N * 4 : 0;
 }
 
 extern "C" int i8l_mxfp4_mm_ws(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,

@@ -257,14 +257,15 @@ py::object quant_per_token(const at::Tensor& x, bool precise_div) {
 // ------------------------------------------------------------------ MXFP4 and the q/k norm
 // Codes [R, K/2] and scales [R, K/32] as the kernels read them without a copy: uint8, unit stride
 // along K, rows that do not share memory.
-bool mx_plain(const at::Tensor& q, const at::Tensor& s, const at::Device& dev) {
+// rows: the dimension of the codes that counts the rows (1: the transposed view of a weight).
+bool mx_plain(const at::Tensor& q, const at::Tensor& s, const at::Device& dev, int rows = 0) {
   if (q.dim() != 2 || s.dim() != 2 || q.scalar_type() != at::kByte || s.scalar_type() != at::kByte ||
       q.device() != dev || s.device() != dev)
     return false;
-  const int64_t r = q.size(0), kb = q.size(1);
+  const int64_t r = q.size(rows), kb = q.size(1 - rows);
   if (kb == 0 || kb % 16 || s.size(0) != r || s.size(1) != kb / 16) return false;
-  return q.stride(1) == 1 && (s.stride(1) == 1 || s.size(1) == 1) &&
-         (r <= 1 || (q.stride(0) >= kb && s.stride(0) >= kb / 16));
+  return q.stride(1 - rows) == 1 && (s.stride(1) == 1 || s.size(1) == 1) &&
+         (r <= 1 || (q.stride(rows) >= kb && s.stride(0) >= kb / 16));
 }
 
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
@@ -354,7 +355,7 @@ py::object mxfp4_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& 
   if (out_code < 0 || !a.is_cuda() || a.dim() != 2 || b.dim() != 2 || a.size(1) != b.size(0))
     return py::none();
   const at::Device dev = a.device();
-  if (!mx_plain(a, sa, dev) || !mx_plain(b.t(), sb, dev)) return py::none();
+  if (!mx_plain(a, sa, dev) || !mx_plain(b, sb, dev, 1)) return py::none();
   const int64_t M = a.size(0), N = b.size(1), K = 2 * a.size(1);
   int32_t bias_code = I8L_DTYPE_NONE;
   const void* bias_ptr = nullptr;
