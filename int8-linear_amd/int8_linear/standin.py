@@ -38,11 +38,15 @@ from __future__ import annotations
 import torch
 
 from int8_linear import fused_quant as fq
+from int8_linear import mxfp4
 from int8_linear.kernel import w8a8_mm
+from int8_linear.qk_rope import qk_norm_rope, rope_cos_sin
 
 HIDDEN = 2048
 INTER = 6144
 Q_COLS = 2048          # q heads x head dim: the slice of qkv that feeds o_proj
+HEAD_DIM, Q_HEADS, KV_HEADS = 128, 16, 8
+ROPE_BASE, MAX_POSITIONS = 1e6, 40960
 LAYERS = 28
 EPS = 1e-6
 # (K, N) of each linear, as vLLM runs Qwen3-1.7B (merged qkv and gate/up)
@@ -186,7 +190,67 @@ class DecoderStandIn:
         return (h, res) if with_residual else h
 
 
-def per_layer_us(stack: DecoderStandIn, windows: int = 5, min_window_ms: float = 20.0,
+class Mxfp4StandIn:
+    """The same decoder with MXFP4 linears, and with the model's norms of the query and key heads and
+    their rotation between qkv_proj and o_proj (the attention is left out here too: the rotated
+    queries go to o_proj, and the rotated keys are returned for a cache).  Per layer:
+
+        add_rmsnorm_mxfp4_quant -> qkv_proj -> qk_norm_rope -> mxfp4_quant -> o_proj
+        -> add_rmsnorm_mxfp4_quant -> gate_up_proj -> silu_mul_mxfp4_quant -> down_proj
+
+    Weights ~ N(0, 0.02) quantized once (26.7 MB a layer), norm weights all ones, x ~ N(0, 1) bf16,
+    positions drawn from a 40960-token context, all from one seeded generator.
+    """
+
+    def __init__(self, m: int, layers: int = LAYERS, seed: int = 0,
+                 device: str | torch.device = "cuda"):
+        g = torch.Generator().manual_seed(seed)
+        dev = torch.device(device)
+        self.m = m
+        self.x = torch.randn((m, HIDDEN), generator=g).to(torch.bfloat16).to(dev)
+        self.positions = torch.randint(0, MAX_POSITIONS, (m,), generator=g).to(dev)
+        self.norm = torch.ones(HIDDEN, dtype=torch.bfloat16, device=dev)
+        self.head_norm = torch.ones(HEAD_DIM, dtype=torch.bfloat16, device=dev)
+        self.cos_sin = rope_cos_sin(MAX_POSITIONS, HEAD_DIM, ROPE_BASE, device=dev)
+        self.layers: list[dict[str, tuple[torch.Tensor, torch.Tensor]]] = []
+        for _ in range(layers):
+            layer = {}
+            for name, (k, n) in SHAPES.items():
+                w = (torch.randn((n, k), generator=g) * 0.02).to(dev)
+                layer[name] = mxfp4.mxfp4_quant(w)
+            self.layers.append(layer)
+
+    def weight_bytes(self) -> int:
+        return sum(w.numel() + s.numel() for layer in self.layers for w, s in layer.values())
+
+    def mm(self, layer, name: str, q: torch.Tensor, s: torch.Tensor) -> torch.Tensor:
+        w, ws = layer[name]
+        return mxfp4.mxfp4_mm(q, w.t(), s, ws, torch.bfloat16)
+
+    def heads(self, qkv: torch.Tensor):
+        """The rotated query and key heads of a qkv_proj output, read in place."""
+        kv = KV_HEADS * HEAD_DIM
+        q = qkv[:, :Q_COLS].unflatten(1, (Q_HEADS, HEAD_DIM))
+        k = qkv[:, Q_COLS:Q_COLS + kv].unflatten(1, (KV_HEADS, HEAD_DIM))
+        return qk_norm_rope(q, k, self.head_norm, self.head_norm, self.cos_sin, self.positions, EPS)
+
+    def forward(self, with_keys: bool = False):
+        """One step through every layer: the last down_proj output [m, HIDDEN], and with_keys the
+        layers' rotated keys."""
+        h, res, keys = self.x, None, []
+        for layer in self.layers:
+            q, s, rout = mxfp4.add_rmsnorm_mxfp4_quant(h, res, self.norm, EPS)
+            res = h if res is None else rout
+            qh, kh = self.heads(self.mm(layer, "qkv_proj", q, s))
+            keys.append(kh)
+            h = self.mm(layer, "o_proj", *mxfp4.mxfp4_quant(qh.flatten(1)))
+            q, s, res = mxfp4.add_rmsnorm_mxfp4_quant(h, res, self.norm, EPS)
+            gu = self.mm(layer, "gate_up_proj", q, s)
+            h = self.mm(layer, "down_proj", *mxfp4.silu_mul_mxfp4_quant(gu))
+        return (h, keys) if with_keys else h
+
+
+def per_layer_us(stack: DecoderStandIn | Mxfp4StandIn, windows: int = 5, min_window_ms: float = 20.0,
                  check=None) -> float:
     """Median microseconds per decoder layer, with the whole step captured as one HIP graph
     and replayed (the reference's discipline, bench/situ_tune.py:127-154).  `check`, if
