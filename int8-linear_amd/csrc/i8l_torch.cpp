@@ -387,7 +387,11 @@ py::object qk_norm_rope(const at::Tensor& q, const at::Tensor& k,
                         const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw,
                         const at::Tensor& cs, const at::Tensor& pos, double eps, bool interleaved,
                         bool inplace) {
-  // (in place goes the Python way, which checks that the heads do not overlap)
+  // (in place goes the Python way, which checks that the heads do not overlap; so does a gradient,
+  // which it refuses)
+  auto grad = [](const c10::optional<at::Tensor>& t) { return t.has_value() && t->requires_grad(); };
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || grad(qw) || grad(kw)))
+    return py::none();
   if (inplace || !q.is_cuda() || q.dim() != 3 || k.dim() != 3 || q.size(0) != k.size(0) ||
       q.size(2) != k.size(2) || k.scalar_type() != q.scalar_type() || q.size(2) < 2 ||
       q.stride(2) != 1 || k.stride(2) != 1)

@@ -110,6 +110,17 @@ def test_python_layer_refuses_host_tensors():
             call()
 
 
+@pytest.mark.parametrize("which", range(4))
+def test_qk_norm_rope_refuses_to_lose_a_gradient(which):
+    args = [torch.zeros(2, 3, 64).bfloat16(), torch.zeros(2, 1, 64).bfloat16(),
+            torch.ones(64).bfloat16(), torch.ones(64).bfloat16()]
+    args[which].requires_grad_()
+    rest = (torch.zeros(8, 64), torch.zeros(2, dtype=torch.int64), 1e-6)
+    for inplace in (False, True):
+        with pytest.raises(NotSupported, match="gradient"):
+            qk_rope.qk_norm_rope(*args, *rest, inplace=inplace)
+
+
 def test_rope_cos_sin_is_exact_far_out():
     t = qk_rope.rope_cos_sin(40960, 64, 1e4, device="cpu")
     assert t.shape == (40960, 64) and t.dtype == torch.float32

@@ -220,3 +220,20 @@ def test_refusals():
             (ValueError, call(q=wide[:1].expand(4, 8, 64), k=k, inplace=True))]:
         with pytest.raises(err):
             f()
+
+
+@pytest.mark.parametrize("which", ["q", "q_weight"])
+def test_a_lost_gradient_is_refused_by_the_binding_too(which):
+    c = _case(4, 2, 1, 64, 64)
+    q, k = _views(c, c["qkv"].cuda())
+    w, rest = c["qw"].cuda(), (c["cs"].cuda(), c["pos"].cuda(), EPS)
+    want = qk_rope.qk_norm_rope(q, k, w, w, *rest)
+    if which == "q":
+        q = q.detach().requires_grad_()
+    else:
+        w = w.clone().requires_grad_()
+    with pytest.raises(NotSupported, match="gradient"):
+        qk_rope.qk_norm_rope(q, k, w, w, *rest)
+    with torch.no_grad():
+        got = qk_rope.qk_norm_rope(q, k, w, w, *rest)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
