@@ -350,6 +350,13 @@ extern "C" int i8l_qk_norm_rope(const void* q, int64_t q_ts, int64_t q_hs, const
            whole(cos_sin) && whole(q_weight) && whole(k_weight);
   };
   const int V = runs(8) ? 8 : runs(4) ? 4 : 0;
+  // a grid's threads stay below 2^32, so its waves at 2^26 less a workgroup's: as many as tokens from
+  // kQkWaves tokens on (launch_qk), else as heads
+  if (T * (V ? 1 : Hq + Hk) > ((int64_t)1 << 26) - 4) {
+    set_error("qk_norm_rope: %lld tokens of %lld + %lld heads of %lld: too large", (long long)T,
+              (long long)Hq, (long long)Hk, (long long)D);
+    return I8L_UNSUPPORTED;
+  }
   const hipStream_t st = (hipStream_t)stream;
   if (V) {
     const int lanes = (int)(R / (2 * V) + (D - R + 2 * V - 1) / (2 * V));

@@ -110,6 +110,14 @@ def test_python_layer_refuses_host_tensors():
             call()
 
 
+@pytest.mark.parametrize("d,t,hk", [(64, (1 << 26) - 3, 0), (6, 1 << 24, 4)])
+def test_qk_norm_rope_refuses_more_waves_than_a_grid_counts(d, t, hk):
+    status = _status(_lib.lib().i8l_qk_norm_rope(P, d, d, P, d * hk, d, P, d, d, P, d * hk, d, None,
+                                                 None, _lib.DTYPE_NONE, 1e-6, P, _lib.F32, 100, P, 64,
+                                                 t, 1, hk, d, d, 0, _lib.BF16, None))
+    assert status == _lib.UNSUPPORTED
+
+
 @pytest.mark.parametrize("which", range(4))
 def test_qk_norm_rope_refuses_to_lose_a_gradient(which):
     args = [torch.zeros(2, 3, 64).bfloat16(), torch.zeros(2, 1, 64).bfloat16(),
