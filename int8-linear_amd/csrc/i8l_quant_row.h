@@ -273,9 +273,8 @@ __device__ __forceinline__ void silu_row(const uint16_t* __restrict__ grow, int 
   // bf16 and fp16 g on gfx950).
   // a = g / d.  For -87 < g < +inf, d is in [1, 7e37], its reciprocal is normal, and one
   // Newton-Markstein correction of g * rcp(d) gives the correctly rounded quotient (checked
-  // against IEEE division for every bf16 and fp16 g in that range on gfx950), up to the
-  // sign of a zero quotient, which no output of this kernel depends on.  A wave holding any
-  // other g recomputes its values with IEEE division.
+  // against IEEE division for every bf16 and fp16 g in that range on gfx950).  A wave holding
+  // any other g recomputes its values with IEEE division.
   // A bf16 SiLU rounded to bf16 (BF16R) needs no exact d: with exp from v_exp_f32, bf16(a) is the
   // same for every bf16 g in that range (checked on gfx950; off by up to 55 fp32 ulps before the
   // rounding, and without the correction of the quotient one gate, 5.9375, rounds the other way).
@@ -309,11 +308,11 @@ __device__ __forceinline__ void silu_row(const uint16_t* __restrict__ grow, int 
                           : canon_expf_core(__builtin_amdgcn_fmed3f(-g[h], -87.5f, 89.5f)));
         const float r0 = __builtin_amdgcn_rcpf(d);
         const float q0 = g[h] * r0;
-        const float e = __builtin_fmaf(-d, q0, g[h]);
-        // the quotient's sign is g's except for g = -0, where the correction gives +0 for
-        // the IEEE -0; the sign of a zero reaches no output (its code is 0 either way, and
-        // absmax takes |y|), so it is not restored here
-        a[h] = __builtin_fmaf(e, r0, q0);
+        // minus the remainder, so that a remainder of zero enters the correction as -0, the
+        // identity of IEEE addition: the quotient of -0 stays -0, which int8 codes do not show
+        // and E2M1 codes do (the remainder g - d q0 itself is +0 there and the sum with it +0)
+        const float e = __builtin_fmaf(d, q0, -g[h]);
+        a[h] = __builtin_fmaf(-e, r0, q0);
         if constexpr (!BF16R) {
           gmin = fminf(gmin, g[h]);
           gmax = fmaxf(gmax, g[h]);
