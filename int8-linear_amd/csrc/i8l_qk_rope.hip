@@ -169,9 +169,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs a, int L, int 
     if (in1) load_floats<V, W32>(a.kw, a.w_dtype, d1, wk[1]);
   }
   // the token's angles; the two runs have the same ones, or V/2 each when interleaved
-  float c[V], s[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) c[i] = 1.0f, s[i] = 0.0f;
+  float c[V] = {}, s[V] = {};
   if (turned) {
     const int64_t at = row * a.R;
     if (row < 0) {
@@ -209,22 +207,24 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(QkArgs a, int L, int 
     for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int i = 0; i < V; ++i) x[r][i] = x[r][i] * rs * (h.q ? wq[r][i] : wk[r][i]);
-    if (INTER) {
+    if (turned) {   // (an angle of 0 would not do: a NaN or an infinity times its sine is a NaN)
+      if constexpr (INTER) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r)
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-          const float ca = c[r * (V / 2) + i / 2], sa = s[r * (V / 2) + i / 2];
-          const float u = x[r][i], v = x[r][i + 1];
-          x[r][i] = __builtin_fmaf(u, ca, -(v * sa));
-          x[r][i + 1] = __builtin_fmaf(v, ca, u * sa);
+          for (int i = 0; i < V; i += 2) {
+            const float ca = c[r * (V / 2) + i / 2], sa = s[r * (V / 2) + i / 2];
+            const float u = x[r][i], v = x[r][i + 1];
+            x[r][i] = __builtin_fmaf(u, ca, -(v * sa));
+            x[r][i + 1] = __builtin_fmaf(v, ca, u * sa);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float u = x[0][i], v = x[1][i];
+          x[0][i] = __builtin_fmaf(u, c[i], -(v * s[i]));
+          x[1][i] = __builtin_fmaf(v, c[i], u * s[i]);
         }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float u = x[0][i], v = x[1][i];
-        x[0][i] = __builtin_fmaf(u, c[i], -(v * s[i]));
-        x[1][i] = __builtin_fmaf(v, c[i], u * s[i]);
       }
     }
     uint16_t* p = (h.q ? qo : ko) + h.i * (int)(h.q ? a.qo_hs : a.ko_hs);
