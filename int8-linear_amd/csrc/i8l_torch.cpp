@@ -268,6 +268,12 @@ bool mx_plain(const at::Tensor& q, const at::Tensor& s, const at::Device& dev, i
          (r <= 1 || (q.stride(rows) >= kb && s.stride(0) >= kb / 16));
 }
 
+// Whether a floating output would lose this input's gradient: the Python way refuses the call.
+bool loses_gradient(const at::Tensor& t) {
+  return at::GradMode::is_enabled() && t.defined() && t.requires_grad();
+}
+bool loses_gradient(const c10::optional<at::Tensor>& t) { return t.has_value() && loses_gradient(*t); }
+
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 py::object mxfp4_quant(const at::Tensor& x, bool round_scale) {
@@ -303,6 +309,7 @@ py::object mxfp4_dequant(const at::Tensor& q, const at::Tensor& s, at::ScalarTyp
 
 py::object add_rmsnorm_mxfp4_quant(const at::Tensor& x, const c10::optional<at::Tensor>& residual,
                                    const at::Tensor& w, double eps, bool round_scale) {
+  if (residual.has_value() && (loses_gradient(x) || loses_gradient(residual))) return py::none();
   if (x.dim() != 2 || !x.is_cuda() || !x.is_contiguous()) return py::none();
   const int32_t act = act_code(x.scalar_type()), wcode = act_code(w.scalar_type());
   const int64_t M = x.size(0), H = x.size(1);
@@ -352,6 +359,7 @@ py::object mxfp4_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& 
                     const at::Tensor& sb, at::ScalarType out_dtype,
                     const c10::optional<at::Tensor>& bias) {
   const int32_t out_code = float_code(out_dtype);
+  if (loses_gradient(bias)) return py::none();
   if (out_code < 0 || !a.is_cuda() || a.dim() != 2 || b.dim() != 2 || a.size(1) != b.size(0))
     return py::none();
   const at::Device dev = a.device();
@@ -389,8 +397,8 @@ py::object qk_norm_rope(const at::Tensor& q, const at::Tensor& k,
                         bool inplace) {
   // (in place goes the Python way, which checks that the heads do not overlap; so does a gradient,
   // which it refuses)
-  auto grad = [](const c10::optional<at::Tensor>& t) { return t.has_value() && t->requires_grad(); };
-  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || grad(qw) || grad(kw)))
+  if (loses_gradient(q) || loses_gradient(k) || loses_gradient(qw) || loses_gradient(kw) ||
+      loses_gradient(cs))
     return py::none();
   if (inplace || !q.is_cuda() || q.dim() != 3 || k.dim() != 3 || q.size(0) != k.size(0) ||
       q.size(2) != k.size(2) || k.scalar_type() != q.scalar_type() || q.size(2) < 2 ||

@@ -63,6 +63,12 @@ def _matrix(codes: torch.Tensor, scales: torch.Tensor, what: str):
     return codes.view(torch.uint8), scales.view(torch.uint8)
 
 
+def _no_gradient(who: str, *inputs: torch.Tensor | None) -> None:
+    """Refuses inputs whose gradient a floating output of `who` would lose."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        raise NotSupported(f"{who} has no gradient: call it under torch.no_grad()")
+
+
 def _ld(t: torch.Tensor) -> int:
     """The row stride; of one row, its length."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -137,10 +143,14 @@ def add_rmsnorm_mxfp4_quant(x: torch.Tensor, residual: torch.Tensor | None, weig
     The values that are quantized are those of fused_quant.add_rmsnorm_quant bit for bit: the
     residual add and the norm in fp32, the normalized value rounded to the weight's dtype, times the
     weight, rounded to x's dtype.  x and residual are contiguous bf16 / fp16 [M, K], weight [K].
+    There is no backward: where gradients are recorded, an x or a residual that requires one is
+    refused with a residual, whose sum with x is returned (codes are integers and have none).
     """
     r = _fast("add_rmsnorm_mxfp4_quant", x, residual, weight, eps, round_scale)
     if r is not None:
         return r
+    if residual is not None:
+        _no_gradient("add_rmsnorm_mxfp4_quant", x, residual)
     act, wcode = _act_code(x, "x"), _act_code(weight, "weight")
     if x.dim() != 2:
         raise ValueError(f"x must be a matrix, got {x.dim()} dimensions")
@@ -199,12 +209,14 @@ def mxfp4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_
 
     a_q [M, K/2] and scale_a [M, K/32] are the activations', scale_b [N, K/32] and b_q = w_q.t()
     [K/2, N] the weight's (codes contiguous along K).  Accumulated in fp32, the bias [N] added in
-    fp32, rounded once.  Rows of codes that start on 16 bytes take the matrix-instruction kernels;
+    fp32, rounded once.  There is no backward: a bias that requires a gradient is refused where
+    gradients are recorded.  Rows of codes that start on 16 bytes take the matrix-instruction kernels;
     any other alignment a slow one of the same results up to the order of the fp32 sums.
     """
     r = _fast("mxfp4_mm", a_q, b_q, scale_a, scale_b, out_dtype, bias)
     if r is not None:
         return r
+    _no_gradient("mxfp4_mm", bias)
     out_code = _float_code(out_dtype, "the output")
     if a_q.dim() != 2 or b_q.dim() != 2 or a_q.shape[1] != b_q.shape[0]:
         raise ValueError(f"cannot multiply codes {tuple(a_q.shape)} by {tuple(b_q.shape)}")

@@ -80,13 +80,14 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     are normalized only.  positions [T] (int32 or int64) picks the rows; a token whose position is
     outside the table gets NaN in its rotated values.  The pairs are (i, i + rot / 2), or
     (2i, 2i + 1) with interleaved.  With inplace, q and k are written over and returned.  There is no
-    backward: heads or weights that require a gradient are refused where gradients are recorded.
+    backward: heads, weights or a table that require a gradient are refused where gradients are
+    recorded.
     """
     r = _fast("qk_norm_rope", q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, inplace)
     if r is not None:
         return r
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad
-                                       for x in (q, k, q_weight, k_weight)):
+                                       for x in (q, k, q_weight, k_weight, cos_sin)):
         raise NotSupported("qk_norm_rope has no gradient: call it under torch.no_grad()")
     act = _heads(q, "q", inplace)
     if _heads(k, "k", inplace) != act:
