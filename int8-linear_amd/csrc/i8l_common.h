@@ -53,23 +53,22 @@ template <int DT>
 __device__ __forceinline__ uint16_t f32_to_act(float v) {
   return DT == I8L_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
 }
-// Round a float through an activation dtype and back (the reference's `.to(dtype).to(f32)`).
-template <int DT>
-__device__ __forceinline__ float round_through(float v) {
-  if (DT == I8L_BF16) return (float)(__bf16)v;
-  return (float)f32_to_f16(v);
-}
-
-// Two values rounded through bf16 with one conversion instruction.
+// Two values rounded to bf16 with one conversion instruction.
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t f32x2_to_bf16x2_bits(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf));
 }
+// The same to fp16 (v_cvt_pk_f16_f32), the values made opaque as in f32_to_f16.
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ v2h f32x2_to_f16x2(float a, float b) {
+  asm("" : "+v"(a), "+v"(b));
+  return __builtin_convertvector((v2f){a, b}, v2h);
+}
 template <int DT>
 __device__ __forceinline__ uint32_t f32x2_to_act2(float a, float b) {
   if (DT == I8L_BF16) return f32x2_to_bf16x2_bits(a, b);
-  return f32_to_f16_bits(a) | ((uint32_t)f32_to_f16_bits(b) << 16);
+  return __builtin_bit_cast(uint32_t, f32x2_to_f16x2(a, b));
 }
 template <int DT>
 __device__ __forceinline__ void round_through2(float& a, float& b) {
@@ -78,9 +77,21 @@ __device__ __forceinline__ void round_through2(float& a, float& b) {
     a = __uint_as_float(p << 16);
     b = __uint_as_float(p & 0xffff0000u);
   } else {
-    a = round_through<DT>(a);
-    b = round_through<DT>(b);
+    const v2h p = f32x2_to_f16x2(a, b);
+    a = (float)p.x;
+    b = (float)p.y;
   }
+}
+// Two values rounded to fp16, times the two fp16 of w, rounded to fp16: the product of two fp16 is
+// exact in fp32, so v_pk_mul_f16's one rounding equals the two of a product in fp32 and its cast.
+__device__ __forceinline__ void round_mul_f16(float& a, float& b, uint32_t w) {
+  const v2h p = f32x2_to_f16x2(a, b) * __builtin_bit_cast(v2h, w);
+  a = (float)p.x;
+  b = (float)p.y;
+}
+// Word i of a 16-byte chunk.
+__device__ __forceinline__ uint32_t chunk_word(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
 // Runtime-dtype forms, for code outside the per-element hot loops.

@@ -147,8 +147,8 @@ __device__ __forceinline__ void store4s(const Epi& e, int64_t m, int64_t n, v4i 
       lo = f32x2_to_bf16x2_bits(o[0], o[1]);
       hi = f32x2_to_bf16x2_bits(o[2], o[3]);
     } else {
-      lo = f32_to_f16_bits(o[0]) | ((uint32_t)f32_to_f16_bits(o[1]) << 16);
-      hi = f32_to_f16_bits(o[2]) | ((uint32_t)f32_to_f16_bits(o[3]) << 16);
+      lo = f32x2_to_act2<I8L_F16>(o[0], o[1]);
+      hi = f32x2_to_act2<I8L_F16>(o[2], o[3]);
     }
     *(uint2*)((uint16_t*)e.out + m * e.ldc + n) = make_uint2(lo, hi);
   }

@@ -931,10 +931,14 @@ gemm_wlds1_dq(const uint16_t* __restrict__ X, int64_t ldx, int64_t up,
         if constexpr (SILU) {
           a0 = silu(a0, ieee);
           a1 = silu(a1, ieee);
-          if constexpr (ACT == kActSiluRound) round_through2<DT>(a0, a1);
-          a0 = a0 * elem(ur[p], k);
-          a1 = a1 * elem(ur[p], k + 1);
-          round_through2<DT>(a0, a1);
+          if constexpr (ACT == kActSiluRound && DT == I8L_F16) {
+            round_mul_f16(a0, a1, chunk_word(ur[p], k / 2));
+          } else {
+            if constexpr (ACT == kActSiluRound) round_through2<DT>(a0, a1);
+            a0 = a0 * elem(ur[p], k);
+            a1 = a1 * elem(ur[p], k + 1);
+            round_through2<DT>(a0, a1);
+          }
         }
         y[p][k] = a0;
         y[p][k + 1] = a1;

@@ -212,10 +212,14 @@ gemm_wlds1p_nq(const uint16_t* __restrict__ X, const uint16_t* __restrict__ R,
 #pragma unroll
     for (int i = 0; i < 8; i += 2) {
       float a = xv[p][i] * rs, b = xv[p][i + 1] * rs;
-      round_through2<DT>(a, b);
-      a = a * gv[i];
-      b = b * gv[i + 1];
-      round_through2<DT>(a, b);
+      if constexpr (DT == I8L_F16) {
+        round_mul_f16(a, b, chunk_word(gr, i / 2));
+      } else {
+        round_through2<DT>(a, b);
+        a = a * gv[i];
+        b = b * gv[i + 1];
+        round_through2<DT>(a, b);
+      }
       xv[p][i] = a;
       xv[p][i + 1] = b;
       am[p] = fmaxf(fmaxf(am[p], fabsf(a)), fabsf(b));   // one max3 with |.| operands

@@ -117,7 +117,7 @@ __device__ __forceinline__ void tile_epilogue(const Epi& e, v16i (&acc)[FA][FB],
     stage([](float x, float y) { return f32x2_to_bf16x2_bits(x, y); });
   else
     stage([](float x, float y) {
-      return (uint32_t)f32_to_f16_bits(x) | ((uint32_t)f32_to_f16_bits(y) << 16);
+      return f32x2_to_act2<I8L_F16>(x, y);
     });
   // Other waves read these stores: the barrier must also wait for them to complete
   // (s_barrier alone does not, and with two workgroups a CU sharing the LDS they do lag).

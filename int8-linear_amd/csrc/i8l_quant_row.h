@@ -101,7 +101,7 @@ __device__ __forceinline__ uint4 load_raw8(const uint16_t* p, int e0, int n) {
 // Elements 2i and 2i+1 of a packed chunk as floats.
 template <int DT>
 __device__ __forceinline__ void unpack_pair(const uint4& v, int i, float& a, float& b) {
-  const uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+  const uint32_t w = chunk_word(v, i);
   if (DT == I8L_BF16) {
     a = __uint_as_float(w << 16);
     b = __uint_as_float(w & 0xffff0000u);
@@ -182,6 +182,17 @@ __device__ __forceinline__ void norm_chunk(float (&xv)[8], float rs, const float
   }
 }
 
+// The same for fp16 rows and weights, the weights as they lie in memory.
+__device__ __forceinline__ void norm_chunk_f16(float (&xv)[8], float rs, const uint4& w) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float a = xv[i] * rs, b = xv[i + 1] * rs;
+    round_mul_f16(a, b, chunk_word(w, i / 2));
+    xv[i] = a;
+    xv[i + 1] = b;
+  }
+}
+
 // The row's normalized values, ready to quantize: x (+ res, written to rout) normalized and scaled
 // by w, rounded as the unquantized norm rounds them.  dsh: kMaxWaves doubles of LDS.
 // J and NW are powers of two, so each wave covers an aligned power-of-two span of the row
@@ -246,6 +257,11 @@ __device__ __forceinline__ void norm_row(const uint16_t* __restrict__ x,
   const float rs = canon_rsqrtf(var + eps);
 #pragma unroll
   for (int j = 0; j < J; ++j) {
+    if constexpr (DT == I8L_F16 && WDT == I8L_F16) {
+      if constexpr (!FULL) wr[j] = load_raw8<VEC>(w, chunk_base<J>(p, j), H);
+      norm_chunk_f16(xv[j], rs, wr[j]);
+      continue;
+    }
     float wv[8];
     if constexpr (FULL)
       unpack8<WDT>(wr[j], wv);
@@ -288,16 +304,35 @@ __device__ __forceinline__ void silu_row(const uint16_t* __restrict__ grow, int 
   typedef short v2s __attribute__((ext_vector_type(2)));
   v2u gu2 = {0, 0};
   v2s gs2 = {0, 0};
+  // fp16 pairs are finished after both ways to their quotients, bf16 ones in each way: the compiler
+  // does not merge the ways where the conversions' asm stands in them, and then keeps every d in
+  // registers for the second (3001 x 14336 fp16, launched over and over: unrounded 52.1 us, so 41.7,
+  // rounded 42.8 and 40.8; in bf16 the one way is as fast as the other)
+  constexpr bool LATE = DT == I8L_F16;
   float gmin = __builtin_inff(), gmax = -__builtin_inff();
+  // y of a pair from its quotients
+  auto finish = [&](int j, int i, float a0, float a1) {
+    if constexpr (ROUND && DT == I8L_F16) {
+      round_mul_f16(a0, a1, chunk_word(uraw[j], i));
+    } else {
+      float u0, u1;
+      unpack_pair<DT>(uraw[j], i, u0, u1);
+      if (ROUND) round_through2<DT>(a0, a1);
+      a0 = a0 * u0;
+      a1 = a1 * u1;
+      round_through2<DT>(a0, a1);
+    }
+    y[j][2 * i] = a0;
+    y[j][2 * i + 1] = a1;
+  };
 #pragma unroll
   for (int j = 0; j < J; ++j)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float g[2], u[2], a[2];
+      float g[2], a[2];
       unpack_pair<DT>(graw[j], i, g[0], g[1]);
-      unpack_pair<DT>(uraw[j], i, u[0], u[1]);
       if constexpr (BF16R) {
-        const uint32_t gw = i == 0 ? graw[j].x : i == 1 ? graw[j].y : i == 2 ? graw[j].z : graw[j].w;
+        const uint32_t gw = chunk_word(graw[j], i);
         gu2 = __builtin_elementwise_max(gu2, __builtin_bit_cast(v2u, gw));
         gs2 = __builtin_elementwise_max(gs2, __builtin_bit_cast(v2s, gw));
       }
@@ -318,12 +353,8 @@ __device__ __forceinline__ void silu_row(const uint16_t* __restrict__ grow, int 
           gmax = fmaxf(gmax, g[h]);
         }
       }
-      if (ROUND) round_through2<DT>(a[0], a[1]);
-      a[0] = a[0] * u[0];
-      a[1] = a[1] * u[1];
-      round_through2<DT>(a[0], a[1]);
-      y[j][2 * i] = a[0];
-      y[j][2 * i + 1] = a[1];
+      if constexpr (LATE) y[j][2 * i] = a[0], y[j][2 * i + 1] = a[1];
+      else finish(j, i, a[0], a[1]);
     }
   bool plain;
   if constexpr (BF16R) {
@@ -338,19 +369,20 @@ __device__ __forceinline__ void silu_row(const uint16_t* __restrict__ grow, int 
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float g[2], u[2], a[2];
+        float g[2], a[2];
         unpack_pair<DT>(graw[j], i, g[0], g[1]);
-        unpack_pair<DT>(uraw[j], i, u[0], u[1]);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           a[h] = g[h] / (1.0f + canon_expf_core(__builtin_amdgcn_fmed3f(-g[h], -87.5f, 89.5f)));
-        if (ROUND) round_through2<DT>(a[0], a[1]);
-        a[0] = a[0] * u[0];
-        a[1] = a[1] * u[1];
-        round_through2<DT>(a[0], a[1]);
-        y[j][2 * i] = a[0];
-        y[j][2 * i + 1] = a[1];
+        if constexpr (LATE) y[j][2 * i] = a[0], y[j][2 * i + 1] = a[1];
+        else finish(j, i, a[0], a[1]);
       }
+  }
+  if constexpr (LATE) {
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) finish(j, i, y[j][2 * i], y[j][2 * i + 1]);
   }
 }
 
