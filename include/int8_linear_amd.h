@@ -398,6 +398,12 @@ int i8l_mxfp4_mm_ws(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb
                     void* stream);
 int64_t i8l_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K);
 
+/* The macro tile (tokens x columns) and the parts of K that i8l_mxfp4_mm_ws launches for contiguous
+ * 16-byte aligned operands with their workspace; 0 x 0 where a kernel for few tokens, or for the
+ * sizes that the macro tiles do not take, runs.  Host-only. */
+int i8l_mxfp4_mm_tile(int64_t M, int64_t N, int64_t K, int32_t* tile_m, int32_t* tile_n,
+                      int32_t* parts);
+
 /*
  * RMSNorm of every query and key head and the rotation of its first R values by the token's
  * position, in fp32 with one rounding:

@@ -63,7 +63,7 @@ __device__ __forceinline__ void mx_store4(const MxMM& p, int64_t m, int64_t n, v
 bool mx_phased_ok(const MxMM& p);
 constexpr int kMaxParts = 8;
 struct MxPhasedPlan {
-  int tile, splits;
+  int tile, splits, bm, bn;   // the tile's index, the parts of K, the tile's rows and columns
 };
 MxPhasedPlan mx_phased_plan(int64_t M, int64_t N, int64_t K, int64_t workspace);
 hipError_t launch_mx_phased(const MxMM& p, void* workspace, int64_t bytes, hipStream_t st);

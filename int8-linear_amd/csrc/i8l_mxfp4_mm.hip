@@ -71,6 +71,23 @@ extern "C" int64_t i8l_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K)
   return splits > 1 ? splits * M * N * 4 : 0;
 }
 
+extern "C" int i8l_mxfp4_mm_tile(int64_t M, int64_t N, int64_t K, int32_t* tile_m, int32_t* tile_n,
+                                 int32_t* parts) {
+  if (!tile_m || !tile_n || !parts) {
+    set_error("mxfp4_mm_tile: an output is NULL");
+    return I8L_INVALID_ARG;
+  }
+  *tile_m = *tile_n = 0;
+  *parts = 1;
+  const bool split = i8l_mxfp4_mm_workspace_bytes(M, N, K) > 0;
+  if (phased_sizes(M, N, K) && M <= INT32_MAX && N <= INT32_MAX && K <= INT32_MAX &&
+      many_tokens(M, N, K, split)) {
+    const MxPhasedPlan plan = mx_phased_plan(M, N, K, split ? kMostWorkspace : 0);
+    *tile_m = plan.bm, *tile_n = plan.bn, *parts = plan.splits;
+  }
+  return I8L_OK;
+}
+
 extern "C" int i8l_mxfp4_mm_ws(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
                                const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b,
                                int64_t ldsb, const void* bias, int32_t bias_dtype, void* out,

@@ -539,7 +539,7 @@ hipError_t launch_mx_phased_tile(int t, int splits, float* parts, const MxMM& p,
 // 4.4 TB/s).  Measured against it (cold weights, us; unsplit / split): 14336 -> 4096 at 128 tokens
 // 30 / 17.8 in 7 parts, at 256 33 / 22.7 in 4, at 512 41.8 / 31.7 in 2; 2048 -> 4096 at 512 6.9 / 18.4.
 MxPhasedPlan mx_phased_plan(int64_t M, int64_t N, int64_t K, int64_t workspace) {
-  MxPhasedPlan best{-1, 1};
+  MxPhasedPlan best{-1, 1, 0, 0};
   double least = 0;
   const int64_t pairs = K / 512;
   const int cus = 256;
@@ -556,7 +556,7 @@ MxPhasedPlan mx_phased_plan(int64_t M, int64_t N, int64_t K, int64_t workspace) 
       if (rest)
         us += steps * (tile.step_idle + (tile.step_full - tile.step_idle) * load) + tile.rest;
       if (s > 1) us += 2.5 + 8.0 * s * M * N / 4.4e6;
-      if (best.tile < 0 || us < least) best = {t, (int)s}, least = us;
+      if (best.tile < 0 || us < least) best = {t, (int)s, tile.bm, tile.bn}, least = us;
     }
   }
   return best;

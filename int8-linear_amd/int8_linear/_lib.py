@@ -39,7 +39,7 @@ EXPORTS = ("i8l_w8a8_mm", "i8l_w8a8_mm_supported", "i8l_default_config", "i8l_la
            "i8l_w8a8_mm_silu_mul", "i8l_w8a8_mm_silu_mul_supported", "i8l_mxfp4_quant",
            "i8l_mxfp4_dequant", "i8l_add_rmsnorm_mxfp4_quant", "i8l_silu_mul_mxfp4_quant",
            "i8l_mxfp4_mm", "i8l_mxfp4_mm_ws", "i8l_mxfp4_mm_workspace_bytes",
-           "i8l_qk_norm_rope", "i8l_last_error", "i8l_version")
+           "i8l_mxfp4_mm_tile", "i8l_qk_norm_rope", "i8l_last_error", "i8l_version")
 
 _lib: ctypes.CDLL | None = None
 
@@ -93,6 +93,7 @@ def lib() -> ctypes.CDLL:
                                _I64, _I64, _I64, _P]
     L.i8l_mxfp4_mm_ws.argtypes = L.i8l_mxfp4_mm.argtypes[:-1] + [_P, _I64, _P]
     L.i8l_mxfp4_mm_workspace_bytes.argtypes = [_I64, _I64, _I64]
+    L.i8l_mxfp4_mm_tile.argtypes = [_I64, _I64, _I64] + [ctypes.POINTER(_I32)] * 3
     L.i8l_qk_norm_rope.argtypes = [_P, _I64, _I64] * 4 + [_P, _P, _I32, ctypes.c_float, _P, _I32,
                                                           _I64, _P, _I32, _I64, _I64, _I64, _I64,
                                                           _I64, _I32, _I32, _P]
