@@ -310,6 +310,13 @@ inline bool operands_ok(const char* who, std::initializer_list<const void*> oper
     }
   return true;
 }
+// Whether a grid along x counts this many waves of 64 lanes, in whole workgroups of up to 16: its
+// threads stay below 2^32; an error naming `who` otherwise.
+inline bool waves_ok(const char* who, int64_t waves) {
+  if (waves <= ((int64_t)1 << 26) - 16) return true;
+  set_error("%s: %lld waves in one launch: too large", who, (long long)waves);
+  return false;
+}
 int hip_status(hipError_t e, const char* where);
 
 }  // namespace i8l

@@ -140,7 +140,8 @@ hipError_t launch_decode_k(const MxMM& p, hipStream_t st) {
 
 bool mx_decode_ok(const MxMM& p) {
   return aligned16(p.a) && aligned16(p.b) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
-         (p.M + 16 * kMaxMT - 1) / (16 * kMaxMT) <= 65535 && p.K <= (int64_t)kStep * INT32_MAX;
+         (p.M + 16 * kMaxMT - 1) / (16 * kMaxMT) <= 65535 && p.K <= (int64_t)kStep * INT32_MAX &&
+         p.N <= ((int64_t)1 << 27) - 16;   // (512 threads for 16 columns: a grid's stay below 2^32)
 }
 
 // Eight waves; the tokens in as few tiles as hold them.

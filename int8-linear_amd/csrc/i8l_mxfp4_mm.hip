@@ -51,6 +51,8 @@ bool many_tokens(int64_t M, int64_t N, int64_t K, bool split) {
   return M > (N >= 20480 ? 32 : N >= 9216 ? 72 : split && K >= 8192 ? 80 : 128);
 }
 
+// Four threads a column (mxfp4_mm_any; the ring's wide launches alike): a grid's stay below 2^32.
+constexpr int64_t kMostColumns = ((int64_t)1 << 30) - 64;
 constexpr int64_t kMostWorkspace = (int64_t)64 << 20;
 
 // The sizes alone of mx_phased_ok.
@@ -64,7 +66,7 @@ bool phased_sizes(int64_t M, int64_t N, int64_t K) {
 using namespace i8l;
 
 extern "C" int64_t i8l_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (!phased_sizes(M, N, K) || M > 4096 || N > INT32_MAX || K > INT32_MAX ||
+  if (!phased_sizes(M, N, K) || M > 4096 || N > kMostColumns || K > INT32_MAX ||
       !many_tokens(M, N, K, true))
     return 0;
   const int splits = mx_phased_plan(M, N, K, kMostWorkspace).splits;
@@ -80,7 +82,7 @@ extern "C" int i8l_mxfp4_mm_tile(int64_t M, int64_t N, int64_t K, int32_t* tile_
   *tile_m = *tile_n = 0;
   *parts = 1;
   const bool split = i8l_mxfp4_mm_workspace_bytes(M, N, K) > 0;
-  if (phased_sizes(M, N, K) && M <= INT32_MAX && N <= INT32_MAX && K <= INT32_MAX &&
+  if (phased_sizes(M, N, K) && M < (int64_t)1 << 30 && N <= kMostColumns && K <= INT32_MAX &&
       many_tokens(M, N, K, split)) {
     const MxPhasedPlan plan = mx_phased_plan(M, N, K, split ? kMostWorkspace : 0);
     *tile_m = plan.bm, *tile_n = plan.bn, *parts = plan.splits;
@@ -103,7 +105,7 @@ extern "C" int i8l_mxfp4_mm_ws(const uint8_t* a, int64_t lda, const uint8_t* b, 
     set_error("mxfp4_mm: the output and the bias must be bf16, fp16 or fp32");
     return I8L_UNSUPPORTED;
   }
-  if (M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) {
+  if (M > INT32_MAX || N > kMostColumns || K > INT32_MAX) {
     set_error("mxfp4_mm: M=%lld N=%lld K=%lld: too large", (long long)M, (long long)N, (long long)K);
     return I8L_UNSUPPORTED;
   }

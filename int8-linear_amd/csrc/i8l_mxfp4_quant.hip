@@ -236,6 +236,9 @@ int chunks_of(int64_t rows, int64_t n) {
 
 bool a4(const void* p) { return ((uintptr_t)p & 3) == 0; }
 
+// Waves of a launch whose waves take j chunks of 512 elements of a row each.
+int64_t waves_of(int64_t rows, int64_t n, int j) { return rows * ((n + 512 * j - 1) / (512 * j)); }
+
 // Checks shared by the entry points: whole blocks, sizes that the grids can count.
 int mx_sizes(const char* who, int64_t M, int64_t K, int64_t most) {
   if (M < 0 || K <= 0 || K % kMxBlock) {
@@ -350,6 +353,7 @@ extern "C" int i8l_mxfp4_quant(const void* x, int64_t ldx, uint8_t* q, uint8_t* 
   const bool one = ldx == K;   // rows that touch are one long row of whole blocks
   const int64_t rows = one ? 1 : M, n = one ? M * K : K;
   const int j = vec ? chunks_of(rows, n) : 1;
+  if (!waves_ok("mxfp4_quant", waves_of(rows, n, j))) return I8L_UNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   switch (x_dtype) {
     case I8L_BF16: launch_mx_quant<I8L_BF16>(j, vec, st, x, ldx, q, scale, rows, n, round_scale); break;
@@ -381,6 +385,7 @@ extern "C" int i8l_mxfp4_dequant(const uint8_t* q, int64_t ldq, const uint8_t* s
   const bool vec = a4(q) && (one || M == 1 || ldq % 4 == 0);
   const int64_t rows = one ? 1 : M, n = one ? M * K : K;
   const int j = vec ? chunks_of(rows, n) : 1;
+  if (!waves_ok("mxfp4_dequant", waves_of(rows, n, j))) return I8L_UNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   switch (out_dtype) {
     case I8L_BF16: launch_mx_dequant<I8L_BF16>(j, vec, st, q, ldq, scale, lds, out, rows, n); break;
@@ -410,6 +415,7 @@ extern "C" int i8l_add_rmsnorm_mxfp4_quant(const void* x, const void* residual, 
   const bool vec = a16(x) && a16(weight) && a4(q) &&
                    (!residual || (a16(residual) && a16(residual_out)));
   const Geom g = norm_geom(M, h, vec);
+  if (!waves_ok("add_rmsnorm_mxfp4_quant", M * g.nw)) return I8L_UNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   auto go = [&](auto launch) {
     launch(g, vec, st, (const uint16_t*)x, (const uint16_t*)residual, (const uint16_t*)weight, eps,
@@ -437,6 +443,7 @@ extern "C" int i8l_silu_mul_mxfp4_quant(const void* gate_up, uint8_t* q, uint8_t
   const int i = (int)I;
   const bool vec = a16(gate_up) && a4(q);
   const int j = vec && M * ((I + 511) / 512) > kSiluWaves ? 2 : 1;
+  if (!waves_ok("silu_mul_mxfp4_quant", waves_of(M, I, j))) return I8L_UNSUPPORTED;
   const hipStream_t st = (hipStream_t)stream;
   if (act_dtype == I8L_BF16)
     launch_mx_silu<I8L_BF16>(j, vec, st, (const uint16_t*)gate_up, q, scale, M, i, round_scale);
