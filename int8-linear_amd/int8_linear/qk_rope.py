@@ -140,6 +140,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
             positions.element_size() * 8, t, hq, hk, d, cos_sin.shape[1], int(bool(interleaved)),
             act, _lib.stream_of(q))
     _lib.check(status, NotSupported)
+    if inplace:   # the kernel writes past autograd, which counts the writes to what it saved
+        torch.autograd.graph.increment_version((q, k))
     return qo, ko
 
 
