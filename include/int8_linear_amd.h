@@ -379,18 +379,22 @@ int i8l_silu_mul_mxfp4_quant(const void* gate_up, uint8_t* q, uint8_t* scale, in
  * out[m,n] = cast(sum_k A[m,k] B[n,k] (+ bias[n])), A [M,K] and B [N,K] MXFP4, accumulated in
  * fp32, one rounding to out_dtype (bf16/f16/f32).  lda, ldb, ldsa, ldsb: bytes from a row of codes
  * or scales to the next; ldc in elements.  bias [N] (bf16/f16/f32) or NULL.  Any alignment; 16-byte
- * aligned rows of codes are the fast ones.  Nothing is allocated.
+ * aligned rows of codes are the fast ones; for many tokens with K a multiple of 512 from 1024 on, N of 8
+ * from 128 on, and every operand and its rows on 16 bytes, scales, bias and out included (elsewhere
+ * the kernels for few tokens run, at 4096 tokens 6 to 13 times as long).  N up to 2^30 - 64.  Nothing
+ * is allocated.
  */
 int i8l_mxfp4_mm(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
                  const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b, int64_t ldsb,
                  const void* bias, int32_t bias_dtype, void* out, int64_t ldc, int32_t out_dtype,
                  int64_t M, int64_t N, int64_t K, void* stream);
 
-/* The same with K split over workgroups where that is faster (some 100 to 512 tokens of a long K):
- * the fp32 partial sums go to the caller's workspace, 16-byte aligned, of at least
- * i8l_mxfp4_mm_workspace_bytes(M, N, K) bytes (0: the call never splits), and a second kernel adds
- * them in order.  A NULL, misaligned or smaller workspace is not used.  Calls that overlap must not
- * share one. */
+/* The same with K split over workgroups where that is faster (products of 33 to 4096 tokens with too
+ * few tiles for the card; 14336 -> 4096: 81 to 640 tokens): the fp32 partial sums go to the caller's
+ * workspace, 16-byte aligned, of at least i8l_mxfp4_mm_workspace_bytes(M, N, K) bytes (0: the call
+ * never splits), and a second kernel adds them in order.  A NULL, misaligned or smaller workspace is
+ * not used.  Calls that overlap must not share one.
+ */
 int i8l_mxfp4_mm_ws(const uint8_t* a, int64_t lda, const uint8_t* b, int64_t ldb,
                     const uint8_t* scale_a, int64_t ldsa, const uint8_t* scale_b, int64_t ldsb,
                     const void* bias, int32_t bias_dtype, void* out, int64_t ldc, int32_t out_dtype,

@@ -10,6 +10,9 @@
 //
 // What bounds it: cache lines, as the lanes of a load hold 16 different rows: 2752 -> 4096 at 1 token
 // 4.2 us, at 64 8.1 (cold weights).  The rows that i8l_mxfp4_ring.hip takes go through LDS instead.
+// It is a kernel for few tokens that also takes many, as the macro tiles need whole 512s of K: every
+// 16 columns read all activations again (2752 -> 4096 at 512 tokens 41.7 us, at 4096 351; the macro
+// tiles at a K of 2560 27 there).
 #include "i8l_mxfp4_mm.h"
 
 namespace i8l {

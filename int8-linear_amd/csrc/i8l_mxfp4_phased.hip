@@ -16,8 +16,8 @@
 //
 // What bounds it: MFMA at the clock its power leaves.  On random operands v_mfma alone reaches 6.4 to
 // 6.7 PFLOP/s (9.9 on zeros); here the MFMAs are busy 60% of the time at 1.76 GHz (68% within a
-// tile's steps, the rest its epilogue): 4096 -> 28672 at 4096 tokens 218 to 227 us, 4.2 to 4.4 PFLOP/s (236 with
-// cold weights), 14336 -> 4096 103 us, 4.7.
+// tile's steps, the rest its epilogue): 4096 -> 28672 at 4096 tokens 215 to 227 us, 4.2 to 4.5 PFLOP/s (236 with
+// cold weights), 1.4 to 1.5 times what the instruction alone would take, 14336 -> 4096 103 us, 4.7.
 #include "i8l_gemm_tile.h"
 #include "i8l_mxfp4_mm.h"
 

@@ -13,7 +13,10 @@
 // cache lines a CU takes from L2 for many, which is why NT grows with the tokens and the columns.
 // 14336 -> 4096 at 80 tokens: 28 us with the fragments loaded straight into registers (a line a
 // lane, as neighbouring lanes hold different rows), 20.7 with each step's 8 bytes of scales copied
-// with it (a line a row again), 15.8 so.
+// with it (a line a row again), 15.8 so.  Many tokens come here where the macro tiles do not take the
+// sizes or the alignment, and read the activations once for every 16 or 32 columns (1792 -> 4096 at 512
+// tokens 19.9 us, at 4096 155, 2048 -> 4096 by macro tiles 8.4 and 22.8; 11008 -> 4096 at 4096 500, of
+// 11264 84).
 #include "i8l_mxfp4_mm.h"
 
 namespace i8l {

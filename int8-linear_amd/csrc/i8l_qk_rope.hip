@@ -14,8 +14,8 @@
 // head that is written over its own input is read whole by the lanes that write it.  A wave takes
 // 64/L heads at a time of one token, whose cos, sin and the two weights stay in its registers; they
 // are loaded 16 bytes at a time, with no choice of type inside (a value at a time, a token of 16 + 8
-// heads takes 6.2 us; so 3.3).  4096 tokens of 32 + 8 heads of 128: 19.7 us, 4.3 TB/s; a copy of as
-// many bytes takes 18.
+// heads takes 6.2 us; so 3.3).  4096 tokens of 32 + 8 heads of 128: 16.2 us over the same rows again and
+// again (5.2 TB/s), 23.2 where rows and outputs change from launch to launch.
 #include <algorithm>
 
 #include "i8l_common.h"
@@ -275,7 +275,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(QkArgs a, int int
 
 // Waves that fill the card: a token's heads are spread over more waves until there are this many (256
 // CUs, 4 SIMDs, 4 waves a SIMD).  More repeat the token's angles and weights: 2048 tokens of 16 + 8
-// heads 8.7 us, at four times the waves 10.1; 4096 of 32 + 8 19.7, at twice 20.3, at four times 23.8.
+// heads 8.7 us, at four times the waves 10.1; 4096 of 32 + 8 19.7, at twice 20.3, at four times 23.8
+// (rows that change from launch to launch).
 constexpr int64_t kQkWaves = 4096;
 
 template <int DT, int V, bool INTER>

@@ -17,8 +17,12 @@ for each call.  Both operands' scales enter the matrix instructions themselves
 (v_mfma_scale_f32_*_f8f6f4), which accumulate in fp32.  A linear reads 17/32 of a byte a weight,
 0.53 of the int8 path's, and the instruction does twice the int8 one's operations.
 
-Launches go on the caller's current stream and allocate nothing but the outputs, and for some
-products of 73 to 512 tokens and a long K the partial sums of its parts.
+Launches go on the caller's current stream and allocate nothing but the outputs, and where a product
+of 33 to 4096 tokens has too few tiles for the card and its K is cut into parts, the parts' sums (up to
+64 MiB; 14336 -> 4096: from 81 to 640 tokens).
+
+There is no backward.  Codes and scales are integers and carry no gradient; a call whose floating
+output would lose one is refused.
 """
 
 from __future__ import annotations
@@ -210,8 +214,13 @@ def mxfp4_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor, scale_
     a_q [M, K/2] and scale_a [M, K/32] are the activations', scale_b [N, K/32] and b_q = w_q.t()
     [K/2, N] the weight's (codes contiguous along K).  Accumulated in fp32, the bias [N] added in
     fp32, rounded once.  There is no backward: a bias that requires a gradient is refused where
-    gradients are recorded.  Rows of codes that start on 16 bytes take the matrix-instruction kernels;
-    any other alignment a slow one of the same results up to the order of the fp32 sums.
+    gradients are recorded.
+
+    Which kernel runs goes by the sizes and the alignment (the same results up to the order of the
+    fp32 sums).  Prompts are fast where K is a multiple of 512 from 1024 on, N of 8 from 128 on, and
+    the codes, the scales, the bias and their rows start on 16 bytes; elsewhere they take the kernels
+    for few tokens, at 4096 tokens 6 to 13 times as long.  Rows of codes that do not start on 16 bytes
+    take a slow kernel without matrix instructions.
     """
     r = _fast("mxfp4_mm", a_q, b_q, scale_a, scale_b, out_dtype, bias)
     if r is not None:
