@@ -10,9 +10,10 @@ import numpy as np
 import pytest
 import torch
 
-from helpers import bits, ints, randn, say
+from helpers import bits, ints, np_, randn, say
 from int8_linear import fused_quant as fq
 from int8_linear import w8a8_mm
+from oracle import oracle as o
 from test_gemm_gpu import oracle_out
 
 pytestmark = pytest.mark.gpu
@@ -63,3 +64,23 @@ def test_silu_mul_quant_takes_about_as_long_as_in_bf16(round_silu, most):
         gu = randn((3001, 2 * 14336), 1, dtype=dtype)
         us[dtype] = _us(lambda: fq.silu_mul_quant(gu, True, round_silu))
     assert us[torch.float16] < most * us[torch.bfloat16], us
+
+
+@pytest.mark.parametrize("m,i", [(5, 6144), (300, 2080)])
+@pytest.mark.parametrize("round_silu", [False, True])
+def test_silu_mul_quant_of_subnormal_products(m, i, round_silu):
+    """SiLU times up below fp16's smallest normal value, 2^-14, down to its last bit."""
+    gu = randn((m, 2 * i), m, 2.0 ** -9, dtype=torch.float16)
+    q, s = fq.silu_mul_quant(gu, True, round_silu)
+    want = o.silu_mul_quant(bits(gu), o.F16, round_silu, True)
+    assert np.array_equal(np_(q), want[0]) and np.array_equal(np_(s), want[1])
+    assert np_(s).max() * 127 < 2.0 ** -14
+
+
+@pytest.mark.parametrize("m,k", [(3, 2048), (5, 2080), (600, 4096), (40, 1000)])
+def test_add_rmsnorm_quant_of_subnormal_products(m, k):
+    x, w = randn((m, k), m, dtype=torch.float16), randn((k,), 3, 2.0 ** -17, dtype=torch.float16)
+    q, s, _ = fq.add_rmsnorm_quant(x, None, w, 1e-6)
+    want = o.add_rmsnorm_quant(bits(x), None, bits(w), 1e-6, o.F16, o.F16)
+    assert np.array_equal(np_(q), want[0]) and np.array_equal(np_(s), want[1])
+    assert np_(s).max() * 127 < 2.0 ** -12

@@ -75,3 +75,23 @@ def test_codes_are_made_of_trained_weights():
     got = mxfp4.add_rmsnorm_mxfp4_quant(x, x, gamma, 1e-6)
     want = mxfp4.add_rmsnorm_mxfp4_quant(x, x, gamma.detach(), 1e-6)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call", ["residual", "bias", "heads"])
+def test_the_custom_ops_have_no_silent_backward(call):
+    """torch records them and raises when the backward comes to them."""
+    ops = torch.ops.int8_linear
+    args = [t.cuda() for t in _norm_args()]
+    if call == "residual":
+        out = ops.add_rmsnorm_mxfp4_quant(args[0], args[1].requires_grad_(), args[2], 1e-6, False)[2]
+    elif call == "bias":
+        bias = torch.ones(4, device="cuda", requires_grad=True)
+        out = ops.mxfp4_mm(*(t.cuda() for t in _mm_args()), torch.float32, bias)
+    else:
+        h = torch.ones(2, 3, 64, device="cuda").bfloat16().requires_grad_()
+        out = ops.qk_norm_rope(h, h[:, :1], None, None, torch.ones(8, 64, device="cuda"),
+                               torch.zeros(2, dtype=torch.int64, device="cuda"), 1e-6, False)[0]
+    assert out.requires_grad
+    with pytest.raises(RuntimeError, match="autograd"):
+        out.float().sum().backward()
