@@ -427,6 +427,63 @@ int i8l_qk_norm_rope(const void* q, int64_t q_ts, int64_t q_hs, const void* k, i
                      int64_t Hq, int64_t Hk, int64_t D, int64_t R, int32_t interleaved,
                      int32_t act_dtype, void* stream);
 
+/*
+ * A layer of E experts of which every token takes k: its router, the order of the (token, choice)
+ * pairs by expert, the W8A8 products over the ordered rows and the sum back to the tokens.  Sizes
+ * and offsets are read on the device, so every call can be captured and replayed with other choices.
+ * No counterpart in the reference, whose linears are dense.
+ *
+ * i8l_moe_route: logits [T,E] (bf16/f16/f32, rows ldl elements apart) to
+ *   experts [T,k]  the k largest logits' experts, largest first, of equal ones the lower expert; a
+ *                  logit of -inf or NaN is never picked (expert -1, weight 0)
+ *   weights [T,k]  scoring 0: softmax, exp(x - max) over its sum; 1: sigmoid, 1 / (1 + exp(-x)).  With
+ *                  renormalize divided by the sum of the picked
+ *   offsets [E+1]  expert e's ordered rows are offsets[e] .. offsets[e+1] - 1
+ *   tokens [T*k]   the token of each ordered row; -1 from row offsets[E] on
+ *   places [T,k]   the ordered row of each pair, -1 for a pair without an expert
+ * Pairs of one expert keep their order (t, then choice).  E up to 512, k up to 64 and E, T*k up to
+ * 2^25.  i8l_moe_order gives the order of experts picked elsewhere: any value outside [0,E) is a pair
+ * without an expert here.  workspace: i8l_moe_order_workspace_bytes(T,E,k) bytes (0: none is needed),
+ * 4-byte aligned, not shared by calls that overlap.
+ */
+int i8l_moe_route(const void* logits, int64_t ldl, int32_t logits_dtype, int64_t T, int64_t E,
+                  int64_t k, int32_t scoring, int32_t renormalize, float* weights, int32_t* experts,
+                  int32_t* offsets, int32_t* tokens, int32_t* places, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+int i8l_moe_order(const int32_t* experts, int64_t T, int64_t E, int64_t k, int32_t* offsets,
+                  int32_t* tokens, int32_t* places, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+int64_t i8l_moe_order_workspace_bytes(int64_t T, int64_t E, int64_t k);
+
+/*
+ * The grouped W8A8 product: for row i of expert e (offsets[e] <= i < offsets[e+1]) and r = rows[i]
+ * (i itself where rows is NULL, and then M == R)
+ *   out[i,n] = cast(f32(sum_k a[r,k] b[e,n,k]) * scale_a[r|0] * scale_b[e,n] (+ bias[e,n]))
+ * a [M,K] int8, rows lda bytes apart; b [E,N,K] int8, experts expert_stride and rows ldb bytes apart;
+ * scale_a M values or one, scale_b and bias (bf16/f16/f32, or NULL) [E,N] contiguous; out [R,N] of
+ * out_dtype (bf16/f16/f32), rows ldc elements apart.  With silu_mul the first N/2 columns are gate
+ * values g, the others up values u, and out [R,N/2] = cast(g / (1 + exp(-g)) * u), all in fp32.
+ * Rows from offsets[E] on are left as they were.  Offsets are held within [0,R] (rows
+ * that none or several name hold anything); an r outside [0,M) gives NaN.  E up to 512, R up to 2^25, K below 2^17.  Any alignment;
+ * fast where K, lda, ldb and expert_stride are multiples of 16, N of 8, and a, b, scale_b, bias and
+ * out and its rows start on 16 bytes.  Nothing is allocated.
+ */
+int i8l_w8a8_grouped_mm(const int8_t* a, int64_t lda, int64_t M, const int32_t* rows,
+                        const int8_t* b, int64_t expert_stride, int64_t ldb, const float* scale_a,
+                        int64_t scale_a_len, const float* scale_b, const void* bias,
+                        int32_t bias_dtype, const int32_t* offsets, void* out, int64_t ldc,
+                        int32_t out_dtype, int32_t silu_mul, int64_t R, int64_t E, int64_t N,
+                        int64_t K, void* stream);
+
+/*
+ * out[t,n] = cast((base[t,n] +) sum_j weights[t,j] * y[places[t,j],n]), j in order, in fp32, one
+ * rounding.  y [R,N] (bf16/f16/f32), base (NULL: none) [T,N] and the contiguous out [T,N] of one
+ * dtype, rows of y and base ldy and ldb elements apart.  A place outside [0,R) adds nothing.
+ */
+int i8l_moe_combine(const void* y, int64_t ldy, int64_t R, const float* weights,
+                    const int32_t* places, const void* base, int64_t ldb, void* out, int64_t T,
+                    int64_t k, int64_t N, int32_t dtype, void* stream);
+
 /* Thread-local description of the last failure ("" if none). */
 const char* i8l_last_error(void);
 

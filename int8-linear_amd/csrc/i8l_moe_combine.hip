@@ -1,0 +1,143 @@
+// The rows of a layer's experts back to their tokens:
+//
+//   out[t, n] = cast( (base[t, n]) + sum_j weights[t, j] * y[places[t, j], n] )
+//
+// in fp32, j in order, one rounding; a place outside [0, R) adds nothing (a pair of no expert here),
+// whatever its weight.
+//
+// Bound by its bytes: k rows of y are read once and one is written.  A thread owns 16 bytes of a
+// token's row, a workgroup up to 256 of them; the loads of kAhead rows are issued before any is used.
+#include "i8l_common.h"
+
+#include <algorithm>
+
+namespace i8l {
+
+namespace {
+
+constexpr int kAhead = 8;
+
+struct Combine {
+  const void* y;
+  int64_t ldy;
+  const float* weights;
+  const int32_t* places;
+  const void* base;
+  int64_t ldb;
+  void* out;
+  int64_t T, N;
+  int R, k;
+};
+
+template <int DT>
+struct Elt { typedef uint16_t type; };
+template <>
+struct Elt<I8L_F32> { typedef float type; };
+
+// V neighbouring elements as they lie in memory.
+template <typename T, int V>
+struct __attribute__((aligned(sizeof(T) * V))) Chunk { T v[V]; };
+
+template <int DT, typename T>
+__device__ __forceinline__ float widen(T v) {
+  if constexpr (DT == I8L_F32) return v;
+  else return act_to_f32<DT>(v);
+}
+
+template <int DT, int V>
+__global__ void __launch_bounds__(256) moe_combine(Combine p) {
+  typedef typename Elt<DT>::type E;
+  typedef Chunk<E, V> Ch;
+  const int64_t t = blockIdx.x;
+  const int64_t n = ((int64_t)blockIdx.y * blockDim.x + threadIdx.x) * V;
+  if (n >= p.N) return;
+  const int32_t* at = p.places + t * p.k;
+  const float* w = p.weights + t * p.k;
+  float acc[V];
+  if (p.base) {
+    const Ch b = *(const Ch*)((const E*)p.base + t * p.ldb + n);
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = widen<DT>(b.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+  }
+  for (int j0 = 0; j0 < p.k; j0 += kAhead) {
+    Ch c[kAhead];
+    float wj[kAhead];
+    bool has[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int row = j0 + j < p.k ? at[j0 + j] : -1;
+      has[j] = row >= 0 && row < p.R;
+      wj[j] = j0 + j < p.k ? w[j0 + j] : 0.0f;
+      if (has[j]) c[j] = *(const Ch*)((const E*)p.y + (int64_t)row * p.ldy + n);
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (has[j]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = acc[i] + wj[j] * widen<DT>(c[j].v[i]);
+      }
+  }
+  Ch o;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (DT == I8L_F32) o.v[i] = acc[i];
+    else o.v[i] = f32_to_act<DT>(acc[i]);
+  }
+  *(Ch*)((E*)p.out + t * p.N + n) = o;
+}
+
+template <int DT, int V>
+hipError_t launch_combine(const Combine& p, hipStream_t st) {
+  const int64_t chunks = (p.N + V - 1) / V;
+  const int block = (int)std::min<int64_t>(256, (chunks + 63) / 64 * 64);
+  const dim3 grid((unsigned)p.T, (unsigned)((chunks + block - 1) / block));
+  hipLaunchKernelGGL((moe_combine<DT, V>), grid, dim3(block), 0, st, p);
+  return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_combine_dt(const Combine& p, hipStream_t st) {
+  constexpr int V = DT == I8L_F32 ? 4 : 8;
+  auto whole = [](const void* q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && ld % V == 0; };
+  const bool vec = p.N % V == 0 && whole(p.y, p.ldy) && whole(p.out, p.N) &&
+                   (!p.base || whole(p.base, p.ldb));
+  return vec ? launch_combine<DT, V>(p, st) : launch_combine<DT, 1>(p, st);
+}
+
+}  // namespace
+}  // namespace i8l
+
+using namespace i8l;
+
+extern "C" int i8l_moe_combine(const void* y, int64_t ldy, int64_t R, const float* weights,
+                               const int32_t* places, const void* base, int64_t ldb, void* out,
+                               int64_t T, int64_t k, int64_t N, int32_t dtype, void* stream) {
+  if (T < 0 || k < 1 || N < 0 || R < 0 || (R > 1 && ldy < N) || (base && T > 1 && ldb < N)) {
+    set_error("moe_combine: bad sizes T=%lld k=%lld N=%lld R=%lld (rows %lld and %lld apart)",
+              (long long)T, (long long)k, (long long)N, (long long)R, (long long)ldy, (long long)ldb);
+    return I8L_INVALID_ARG;
+  }
+  if (dtype != I8L_BF16 && dtype != I8L_F16 && dtype != I8L_F32) {
+    set_error("moe_combine: bf16, fp16 or fp32 only");
+    return I8L_UNSUPPORTED;
+  }
+  // a grid counts its threads below 2^32 along x and 65535 workgroups along y
+  if (T > ((int64_t)1 << 24) - 1 || N > (int64_t)65535 * 256 || R > INT32_MAX || k > 1024) {
+    set_error("moe_combine: T=%lld k=%lld N=%lld R=%lld: too large", (long long)T, (long long)k,
+              (long long)N, (long long)R);
+    return I8L_UNSUPPORTED;
+  }
+  if (T == 0 || N == 0) return I8L_OK;
+  if (!operands_ok("moe_combine", {weights, places, out}) ||
+      (R > 0 && !operands_ok("moe_combine", {y})))
+    return I8L_INVALID_ARG;
+  const Combine p{y, ldy, weights, places, base, ldb, out, T, N, (int)R, (int)k};
+  const hipStream_t st = (hipStream_t)stream;
+  const hipError_t e = dtype == I8L_BF16  ? launch_combine_dt<I8L_BF16>(p, st)
+                       : dtype == I8L_F16 ? launch_combine_dt<I8L_F16>(p, st)
+                                          : launch_combine_dt<I8L_F32>(p, st);
+  return hip_status(e, "moe_combine launch");
+}
