@@ -47,17 +47,6 @@ __device__ __forceinline__ void expert_rows(const Grouped& p, int e, int& lo, in
   hi = min(max(p.offsets[e + 1], lo), p.R);
 }
 
-// Inclusive sum over the 64 lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);   // row_bcast 15, 31
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);
-  return v;
-}
-
 // A tile: rows [row0, end) of expert e (up to bm of them), column block `col`.
 struct GroupTile {
   int e, row0, end, col;
@@ -153,5 +142,8 @@ __device__ __forceinline__ float group_silu(const Grouped& p, float g, float u) 
 
 // Any alignment, any K and N (i8l_grouped_mm.hip).
 hipError_t launch_grouped_any(const Grouped& p, hipStream_t st);
+// Macro tiles of bm = 64, 128 or 256 rows x 256 columns (i8l_grouped_phased.hip).
+bool grouped_phased_ok(const Grouped& p);
+hipError_t launch_grouped_phased(int bm, const Grouped& p, hipStream_t st);
 
 }  // namespace i8l

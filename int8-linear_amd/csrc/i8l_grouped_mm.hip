@@ -95,6 +95,12 @@ hipError_t launch_any_v(const Grouped& p, hipStream_t st) {
   return hipGetLastError();
 }
 
+// The rows of a macro tile, by the rows an expert has on average.
+int phased_rows(int64_t R, int64_t E) {
+  const int64_t each = R / E;
+  return each <= 48 ? 64 : each <= 512 ? 128 : 256;
+}
+
 }  // namespace
 
 hipError_t launch_grouped_any(const Grouped& p, hipStream_t st) {
@@ -156,5 +162,7 @@ extern "C" int i8l_w8a8_grouped_mm(const int8_t* a, int64_t lda, int64_t M, cons
   p.sa_per_row = scale_a_len != 1, p.bias_dtype = bias ? bias_dtype : I8L_DTYPE_NONE;
   p.out_dtype = out_dtype, p.silu = silu_mul != 0;
   const hipStream_t st = (hipStream_t)stream;
-  return hip_status(launch_grouped_any(p, st), "w8a8_grouped_mm launch");
+  const hipError_t e = grouped_phased_ok(p) ? launch_grouped_phased(phased_rows(R, E), p, st)
+                                            : launch_grouped_any(p, st);
+  return hip_status(e, "w8a8_grouped_mm launch");
 }

@@ -1,0 +1,510 @@
+// Macro tiles of the grouped W8A8 product, for experts with many rows: persistent workgroups whose K
+// steps are cut into four phases, one per quadrant of a wave's tile (v_mfma_i32_32x32x32_i8).
+#include "i8l_gemm_tile.h"
+#include "i8l_grouped.h"
+
+namespace i8l {
+
+namespace {
+
+// ------------------------------------------------------------------ schedule
+// A workgroup of 4 waves (WM x WN, one a SIMD) computes BM x BN tiles in 128-byte K steps.  A wave's
+// tile is 2 x 2 quadrants of 32 x 32 fragments: its rows are an A half 0 and 1 of QA fragments each,
+// its columns a B half 0 and 1 of QB each, and the LDS holds each operand's step as those two halves
+// in two buffers.  With SILU the B half 0 is gate columns and half 1 the up columns of the same
+// indices, so a lane ends with both factors of its outputs.
+//
+// Step t is four phases, with f = t % 2 and s = 1 - f (the order of the B halves alternates):
+//   phase 0: MFMAs of (A0, Bf);   reads Bs(t);     requests A0(t+2)
+//   phase 1: MFMAs of (A0, Bs);   reads A1(t);     requests Bf(t+2)
+//   phase 2: MFMAs of (A1, Bs);   reads A0(t+1);   requests Bs(t+2)
+//   phase 3: MFMAs of (A1, Bf);   reads Bs(t+1), which is t+1's first;  requests A1(t+2)
+// so every fragment is read from LDS once a step and a phase before its use, and the copies of a step
+// go out a quarter a phase, each into the half whose reads ended a phase before, six phases before it
+// is read.  Each phase ends with lgkmcnt(0) (this wave's reads are done: that half may be refilled),
+// vmcnt (all but the newest five halves have landed: the next phase's reads) and one workgroup
+// barrier, which makes both true of every wave.
+//
+// The workgroups walk the tiles of all experts; the copies of a tile's last two steps are the next
+// tile's first two, so they fly during the epilogue, which every wave does alone through its own 4 KiB
+// of LDS.  What a tile needs to be found stands in LDS: the experts' first blocks and rows, and the
+// source rows of three tiles (read an epilogue ahead, where nothing but stores is in flight, so that
+// no wait for them drains the copies).
+//
+// The copies are buffer loads with the row's byte offset in a register and the K position in a scalar:
+// an offset past the buffer's size reads as zeros, which gives rows past the expert's last, whole
+// steps past K and its tail within a step their zeros at the price of one instruction a copy (zeros
+// toggle nothing: they cost little of the power that bounds the multiplications).
+constexpr int kStep = 128;
+constexpr uint32_t kOutside = 0x80000000u;   // (the buffers are smaller than 2^31 bytes)
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+// A buffer of `bytes` bytes from p on, checked byte by byte (raw, no stride).
+__device__ __forceinline__ v4u buffer_of(const void* p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  return v4u{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) & 0xffffu,
+             (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
+}
+
+// 16 bytes a lane into 1 KiB of LDS from `dst` on.  Assembly, so that the compiler, which cannot count
+// these among other requests, places no wait of its own: the phases' explicit waits cover them.
+__device__ __forceinline__ void copy_1k(v4u buf, uint32_t off, int at, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+               ::"v"(off), "s"(buf), "s"(at), "s"(dst) : "memory", "m0");
+}
+
+// The scales and bias of 4 neighbouring columns of an expert (past the last: the last four's).
+struct ColQuad {
+  float sb[4], bias[4];
+};
+template <bool BIAS>
+__device__ __forceinline__ ColQuad load_quad(const Grouped& p, int64_t at, int n) {
+  n = min(n, p.N - 4);
+  ColQuad c;
+  const float4 s = *(const float4*)(p.sb + at + n);
+  c.sb[0] = s.x, c.sb[1] = s.y, c.sb[2] = s.z, c.sb[3] = s.w;
+  if constexpr (BIAS) {
+    if (p.bias_dtype == I8L_F32) {
+      const float4 b = *(const float4*)((const float*)p.bias + at + n);
+      c.bias[0] = b.x, c.bias[1] = b.y, c.bias[2] = b.z, c.bias[3] = b.w;
+    } else {
+      const uint2 h = *(const uint2*)((const uint16_t*)p.bias + at + n);
+      const uint32_t w[4] = {h.x & 0xffffu, h.x >> 16, h.y & 0xffffu, h.y >> 16};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c.bias[r] = act_to_f32(w[r], p.bias_dtype);
+    }
+  }
+  return c;
+}
+
+struct PhasedShared {
+  int32_t first[kMaxExperts + 1];            // an expert's first block; [E]: their number
+  int32_t lo[kMaxExperts], hi[kMaxExperts];  // its rows
+  int32_t source[3][256];                    // a tile's rows of A; -1: past the expert's last
+};
+
+constexpr int kBadRow = -2;   // a source row outside [0, M): zeros, and NaN in the end
+
+template <int WM, int QA, int QB, int OD, bool BIAS, bool SILU>
+__global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes, uint32_t bbytes, int steps) {
+  constexpr int W = 4, WN = W / WM;
+  constexpr int QN = 2 * QB;                         // column fragments of a wave
+  constexpr int BM = WM * 64 * QA, BN = WN * 32 * QN, BK = kStep;
+  constexpr int BNO = SILU ? BN / 2 : BN;            // output columns
+  constexpr int CPR = BK / 16, RPC = 64 / CPR;       // chunks of a row, rows of a copy
+  constexpr int KK = BK / 32;                        // MFMA substeps of a step
+  constexpr int HA = BM / 2 * BK, HB = BN / 2 * BK;  // bytes of a half
+  constexpr int JA = HA / 1024 / W, JB = HB / 1024 / W;   // copies a wave
+  constexpr int B0 = 4 * HA, SB = 2 * HB;            // LDS: A [buffer][half], then B, then staging
+  constexpr int STG = B0 + 2 * SB;
+  static_assert(JA >= 1 && JB >= 1 && BM <= 256, "whole copies");
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+  PhasedShared& sh = *(PhasedShared*)(lds + STG + W * 4096);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int width = SILU ? p.N / 2 : p.N;            // output columns of the problem
+  const int cols = (width + BNO - 1) / BNO;
+  const int KT = steps;
+
+  // ---- the experts' blocks
+  if (wave == 0) {
+    const int per = (p.E + 63) / 64, e0 = min(lane * per, p.E), e1 = min(e0 + per, p.E);
+    int blocks = 0;
+    for (int e = e0; e < e1; ++e) {
+      int lo, hi;
+      expert_rows(p, e, lo, hi);
+      sh.lo[e] = lo;
+      sh.hi[e] = hi;
+      sh.first[e] = blocks;
+      blocks += (hi - lo + BM - 1) / BM;
+    }
+    const int upto = wave_scan(blocks);
+    for (int e = e0; e < e1; ++e) sh.first[e] += upto - blocks;
+    if (lane == 63) sh.first[p.E] = upto;
+  }
+  __syncthreads();
+  const int total_blocks = __builtin_amdgcn_readfirstlane(sh.first[p.E]);
+  const int64_t total64 = (int64_t)total_blocks * cols;
+  const int tiles = (int)min(total64, (int64_t)INT32_MAX);
+  if ((int)blockIdx.x >= tiles) return;
+
+  // Tile `t` of this walk: consecutive positions go to one XCD, and within an expert up to 8 row blocks
+  // are walked together, so that what runs at a time shares weight and activation rows in L2.
+  auto tile_at = [&](int t) {
+    const int pos = xcd_order(t, tiles);
+    const int q = pos / cols;
+    const int per = (p.E + 63) / 64;
+    const uint64_t m1 = __ballot(sh.first[min((lane + 1) * per, p.E)] > q);
+    const int g = __builtin_ctzll(m1) * per;
+    const uint64_t m2 = __ballot(sh.first[min(g + lane + 1, p.E)] > q);
+    GroupTile o;
+    o.e = __builtin_amdgcn_readfirstlane(g + __builtin_ctzll(m2));
+    const int f = __builtin_amdgcn_readfirstlane(sh.first[o.e]);
+    const int nb = __builtin_amdgcn_readfirstlane(sh.first[o.e + 1]) - f;
+    const int lo = __builtin_amdgcn_readfirstlane(sh.lo[o.e]);
+    const int hi = __builtin_amdgcn_readfirstlane(sh.hi[o.e]);
+    const int local = pos - f * cols;
+    constexpr int GM = 8;
+    const int first = local / (GM * cols) * GM, gsize = min(nb - first, GM);
+    const int in = local - first * cols;
+    o.col = in / gsize;
+    o.row0 = lo + (first + in % gsize) * BM;
+    o.end = min(o.row0 + BM, hi);
+    return o;
+  };
+  // a tile's source rows: row tid of it
+  auto source_of = [&](const GroupTile& g) {
+    if (tid >= BM) return -1;
+    const int i = g.row0 + tid;
+    if (i >= g.end) return -1;
+    const int r = p.rows ? p.rows[i] : i;
+    return r >= 0 && r < p.M ? r : kBadRow;
+  };
+
+  // Copies: copy j of a half writes LDS rows [RPC x, RPC x + RPC), x = W j + wave; lane l writes
+  // slot l % CPR of row l / CPR.  Half row r lies in wave block r / R of that half (R rows each).
+  const int lrow = lane / CPR;
+  const int chunk = ((lane % CPR) ^ swz<BK>(wave * RPC + lrow)) * 16;
+  static_assert((W * RPC) % 16 == 0, "the swizzle must not depend on j");
+  const int lda32 = (int)p.lda, ldb32 = (int)p.ldb;
+  int arow[2][JA], brow[2][JB];   // tile rows; the weight's byte offsets in the tile being requested
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int j = 0; j < JA; ++j) {
+      constexpr int RA = 32 * QA;
+      const int r = (W * j + wave) * RPC;
+      arow[h][j] = (r / RA) * (2 * RA) + h * RA + r % RA;
+    }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_i8*)lds + wave * 1024;
+  const uint32_t voffB = (uint32_t)(lrow * ldb32 + chunk);
+  const v4u bufA = buffer_of(p.a, abytes);
+  v4u bufB = bufA;
+  uint32_t voffA[2][JA];
+  int kreq = 0;            // the K position being requested
+  uint32_t past = 0;       // kOutside in the lanes whose chunk of that step lies past K
+  auto request_from = [&](const GroupTile& g, int buf) {
+    bufB = buffer_of(p.b + g.e * p.eb, bbytes);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < JA; ++j) {
+        const int r = sh.source[buf][arow[h][j] + lrow];
+        voffA[h][j] = r >= 0 ? (uint32_t)(r * lda32 + chunk) : kOutside;
+      }
+      constexpr int RB = 32 * QB;
+#pragma unroll
+      for (int j = 0; j < JB; ++j) {
+        // eight columns, all within the problem or all past it (then the last eight again, not stored)
+        const int r = (W * j + wave) * RPC, x = r / RB, y = r % RB;
+        const int n = SILU ? h * width + min(g.col * BNO + x * RB + y, width - 8)
+                           : min(g.col * BN + x * (2 * RB) + h * RB + y, width - 8);
+        brow[h][j] = n * ldb32;
+      }
+    }
+    kreq = 0;
+  };
+  auto begin_step = [&] { past = kreq + chunk < p.K ? 0u : kOutside; };
+  // copy j of A's / B's half h of the step being requested, into buffer buf
+  auto copyA = [&](int h, int buf, int j) {
+    copy_1k(bufA, voffA[h][j] | past, kreq, lds0 + (2 * buf + h) * HA + j * 1024 * W);
+  };
+  auto copyB = [&](int h, int buf, int j) {
+    copy_1k(bufB, voffB | past, kreq + brow[h][j], lds0 + B0 + buf * SB + h * HB + j * 1024 * W);
+  };
+
+  // Fragment reads: lane l reads row l%32 of a 32-row block, chunk 2*kk + l/32.
+  const int frow = lane & 31, fhalf = lane >> 5;
+  int ofs[KK];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) ofs[kk] = frow * BK + (((2 * kk + fhalf) ^ swz<BK>(frow)) * 16);
+  const int8_t* la = lds + wm * 32 * QA * BK;
+  const int8_t* lb = lds + B0 + wn * 32 * QB * BK;
+  v4i fa[2][QA][KK], fb[2][QB][KK];
+  auto readA = [&](int h, int buf, int kk) {
+#pragma unroll
+    for (int i = 0; i < QA; ++i)
+      fa[h][i][kk] = *(const v4i*)(la + ofs[kk] + (2 * buf + h) * HA + i * 32 * BK);
+  };
+  auto readB = [&](int h, int buf, int kk) {
+#pragma unroll
+    for (int i = 0; i < QB; ++i)
+      fb[h][i][kk] = *(const v4i*)(lb + ofs[kk] + buf * SB + h * HB + i * 32 * BK);
+  };
+
+  v16i acc[2][2][QA][QB];
+  // A phase's work: per MFMA substep its MFMAs with the next phase's reads of that substep between
+  // them, and one in KK of its copies.  zero: a tile's first step, whose first substep starts from 0.
+  auto body = [&](auto hac, auto hbc, auto zero, auto read, int reads, auto copy, auto copies) {
+    constexpr int ha = decltype(hac)::value, hb = decltype(hbc)::value;
+    constexpr int NC = decltype(copies)::value;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+#pragma unroll
+      for (int i = 0; i < QA; ++i)
+#pragma unroll
+        for (int j = 0; j < QB; ++j)
+          acc[ha][hb][i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+              fb[hb][j][kk], fa[ha][i][kk],
+              decltype(zero)::value && kk == 0 ? v16i{} : acc[ha][hb][i][j], 0, 0, 0);
+      read(kk);
+#pragma unroll
+      for (int j = kk * NC / KK; j < (kk + 1) * NC / KK; ++j) copy(j);
+#pragma unroll
+      for (int i = 0; i < QA * QB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                 // one MFMA
+        if (i < reads) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // one LDS read
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // One K step of parity `par`.  TAIL: a tile's last (it reads nothing ahead).  HEAD: 4 for a
+  // tile's first step and 1 for its second, the phases that `landed` spares the wait for copies
+  // (a workgroup's later tiles find them landed).
+  typedef std::integral_constant<int, 0> I0;
+  typedef std::integral_constant<int, 1> I1;
+  typedef std::integral_constant<int, JA> NJA;
+  typedef std::integral_constant<int, JB> NJB;
+  auto step = [&](auto par, auto tail, auto headc, bool landed) {
+    constexpr int f = decltype(par)::value, s = 1 - f;
+    constexpr bool TAIL = decltype(tail)::value;
+    constexpr int HEAD = decltype(headc)::value;
+    constexpr std::bool_constant<HEAD == 4> zero{};
+    typedef std::integral_constant<int, f> HF;
+    typedef std::integral_constant<int, s> HS;
+    constexpr int NA = 3 * JA + 2 * JB, NB = 2 * JA + 3 * JB;
+    auto phase_end = [&](auto phasec, auto nc) {
+      constexpr int phase = decltype(phasec)::value, N = decltype(nc)::value;
+      if constexpr (phase < HEAD) {
+        wait_lgkmcnt0();
+        if (!landed) wait_vmcnt<N>();
+      } else {
+        wait_vmcnt_lgkm0<N>();
+      }
+      lds_barrier();
+    };
+    begin_step();
+    body(I0{}, HF{}, zero, [&](int kk) { readB(s, f, kk); }, QB, [&](int j) { copyA(0, f, j); }, NJA{});
+    phase_end(I0{}, std::integral_constant<int, NA>{});
+    body(I0{}, HS{}, zero, [&](int kk) { readA(1, f, kk); }, QA, [&](int j) { copyB(f, f, j); }, NJB{});
+    phase_end(I1{}, std::integral_constant<int, NB>{});
+    body(I1{}, HS{}, zero, [&](int kk) { if constexpr (!TAIL) readA(0, 1 - f, kk); }, TAIL ? 0 : QA,
+         [&](int j) { copyB(s, f, j); }, NJB{});
+    if constexpr (!TAIL) phase_end(std::integral_constant<int, 2>{}, std::integral_constant<int, NB>{});
+    body(I1{}, HF{}, zero, [&](int kk) { if constexpr (!TAIL) readB(s, 1 - f, kk); }, TAIL ? 0 : QB,
+         [&](int j) { copyA(1, f, j); }, NJA{});
+    if constexpr (!TAIL) phase_end(std::integral_constant<int, 3>{}, std::integral_constant<int, NA>{});
+    kreq += BK;
+  };
+  auto request_step = [&](auto par) {   // a whole step, in the order the phases request it
+    constexpr int f = decltype(par)::value, s = 1 - f;
+    begin_step();
+    for (int j = 0; j < JA; ++j) copyA(0, f, j);
+    for (int j = 0; j < JB; ++j) copyB(f, f, j);
+    for (int j = 0; j < JB; ++j) copyB(s, f, j);
+    for (int j = 0; j < JA; ++j) copyA(1, f, j);
+    kreq += BK;
+  };
+
+  int tile = blockIdx.x, buf = 0;   // buf: where the tile's source rows stand
+  GroupTile g0 = tile_at(tile), g1 = g0;
+  bool more = tile + (int)gridDim.x < tiles;   // (tile + gridDim.x stays below 2^31: see the launch)
+  if (more) g1 = tile_at(tile + gridDim.x);
+  if (tid < BM) {
+    sh.source[0][tid] = source_of(g0);
+    sh.source[1][tid] = source_of(g1);
+  }
+  __syncthreads();
+  request_from(g0, 0);
+  request_step(I0{});
+  request_step(I1{});
+  bool landed = false;
+  for (;;) {
+    // A0(0) and B0(0) into registers, then the steps in pairs, the first and the last apart
+    if (!landed) wait_vmcnt<3 * JA + 3 * JB>();
+    lds_barrier();
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      readA(0, 0, kk);
+      readB(0, 0, kk);
+    }
+    wait_lgkmcnt0();
+    if (!landed) wait_vmcnt<3 * JA + 2 * JB>();
+    lds_barrier();
+
+    // the copies awaited in the first five phases were requested before the previous tile's
+    // stores, whose epilogue waited for them
+    step(I0{}, std::false_type{}, std::integral_constant<int, 4>{}, landed);
+    step(I1{}, std::false_type{}, I1{}, landed);
+    for (int t = 2; t + 2 < KT; t += 2) {
+      step(I0{}, std::false_type{}, I0{}, false);
+      step(I1{}, std::false_type{}, I0{}, false);
+    }
+    const int buf1 = buf == 2 ? 0 : buf + 1, buf2 = buf1 == 2 ? 0 : buf1 + 1;
+    request_from(g1, buf1);   // (past the last tile: one of its rows again, not used)
+    step(I0{}, std::false_type{}, I0{}, false);
+    step(I1{}, std::true_type{}, I0{}, false);
+
+    // ---- epilogue: acc * scale_a * scale_b (+ bias) in fp32, left to right, then one cast.
+    // Each wave takes 32 rows x 64 columns (16-bit outputs; 32 columns of 4-byte ones) at a time
+    // through its 4 KiB: rows of 128 bytes, chunk c at slot c ^ (row & 7), written out in whole
+    // 128-byte lines, 8 rows a store.  The lane index is taken anew, opaque, so that what the
+    // epilogue derives from it is not kept in registers over the main loop.
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int erow = ln & 31, ehalf = ln >> 5, srow = ln >> 3, sch = ln & 7;
+    constexpr int FN = SILU ? QB : QN;                // output fragments across
+    const int nw = g0.col * BNO + wn * 32 * FN, mw = wm * 64 * QA;
+    int8_t* stg = lds + STG + wave * 4096;
+    const int64_t ecol = (int64_t)g0.e * p.N;
+    float sam[2][QA];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < QA; ++i) {
+        const int r = sh.source[buf][mw + (h * QA + i) * 32 + erow];
+        const float s = p.sa[p.sa_per_row ? max(r, 0) : 0];
+        sam[h][i] = r == kBadRow ? __builtin_nanf("") : s;
+      }
+    // every copy in flight (the next tile's first two steps) has landed past here, so the next
+    // tile's first waits need not count past this tile's stores
+    wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    // the tile after the next one, and its source rows
+    const bool more2 = more && tile + 2 * (int64_t)gridDim.x < tiles;
+    GroupTile g2 = g1;
+    if (more2) g2 = tile_at(tile + 2 * gridDim.x);
+    const int src2 = source_of(g2);
+    constexpr int FG = OD == I8L_F32 ? 1 : 2;         // fragments at a time
+#pragma unroll
+    for (int x0 = 0; x0 < FN; x0 += FG) {
+      constexpr int PER = FN < FG ? FN : FG;
+      ColQuad cl[PER][4], cu[SILU ? PER : 1][4];
+#pragma unroll
+      for (int c = 0; c < PER; ++c)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = nw + 32 * (x0 + c) + 8 * q + 4 * ehalf;
+          cl[c][q] = load_quad<BIAS>(p, ecol, SILU ? min(n, width - 4) : n);
+          if constexpr (SILU) cu[c][q] = load_quad<BIAS>(p, ecol, width + min(n, width - 4));
+        }
+      auto scaled = [&](int32_t a, float sa, const ColQuad& c, int r) {
+        float v = (float)a;
+        v = v * sa;
+        v = v * c.sb[r];
+        if constexpr (BIAS) v = v + c.bias[r];
+        return v;
+      };
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < QA; ++i) {
+          const int mb = g0.row0 + mw + (h * QA + i) * 32;
+#pragma unroll
+          for (int c = 0; c < PER; ++c) {
+            const int x = x0 + c;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float v[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                if constexpr (SILU) {
+                  v[r] = silu_mul<OD == I8L_F32>(
+                      scaled(acc[h][0][i][x][4 * q + r], sam[h][i], cl[c][q], r),
+                      scaled(acc[h][1][i][x][4 * q + r], sam[h][i], cu[c][q], r));
+                } else {
+                  v[r] = scaled(acc[h][x / QB][i][x % QB][4 * q + r], sam[h][i], cl[c][q], r);
+                }
+                // the value itself is rounded to fp16 in a cast of its own: opaque, or the product
+                // and the cast become one v_fma_mixlo_f16, which rounds once
+                if constexpr (OD == I8L_F16) asm volatile("" : "+v"(v[r]));
+              }
+              if constexpr (OD == I8L_F32)
+                *(float4*)(stg + erow * 128 + (((2 * q + ehalf) ^ (erow & 7)) * 16)) =
+                    make_float4(v[0], v[1], v[2], v[3]);
+              else
+                *(uint2*)(stg + erow * 128 + (((4 * c + q) ^ (erow & 7)) * 16) + 8 * ehalf) =
+                    make_uint2(f32x2_to_act2<OD>(v[0], v[1]), f32x2_to_act2<OD>(v[2], v[3]));
+            }
+          }
+          constexpr int EPC = OD == I8L_F32 ? 4 : 8;   // elements of a chunk
+          const int n = nw + 32 * x0 + EPC * sch;
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const int row = 8 * y + srow;
+            const v4i v = *(const v4i*)(stg + row * 128 + ((sch ^ srow) * 16));
+            if (mb + row < g0.end && n < width && sch * EPC < 32 * PER)
+              __builtin_nontemporal_store(
+                  v, (v4i*)((char*)p.out + ((mb + row) * p.ldc + n) * (OD == I8L_F32 ? 4 : 2)));
+          }
+        }
+      asm volatile("" ::: "memory");   // the next columns' operands load after these
+    }
+    if (!more) break;
+    if (tid < BM) sh.source[buf2][tid] = src2;
+    tile += gridDim.x;
+    buf = buf1;
+    more = more2;
+    g0 = g1;
+    g1 = g2;
+    landed = true;
+  }
+}
+
+// ------------------------------------------------------------------ host side
+template <int WM, int QA, int QB, int OD, bool BIAS, bool SILU>
+hipError_t launch_k(const Grouped& p, hipStream_t st) {
+  auto kern = grouped_phased<WM, QA, QB, OD, BIAS, SILU>;
+  constexpr int BM = WM * 64 * QA, BN = (4 / WM) * 64 * QB;
+  constexpr size_t shm = 2 * (size_t)(BM + BN) * kStep + 4 * 4096 + sizeof(PhasedShared);
+  static_assert(shm <= kMaxLds, "two buffers, the staging and the tables fit the LDS");
+  static std::atomic<uint64_t> lds_done{0};  // devices this kernel is opted in on
+  lds_opt_in((const void*)kern, shm, lds_done);
+  const int width = SILU ? p.N / 2 : p.N, bno = SILU ? BN / 2 : BN;
+  const int64_t tiles = most_blocks(p.R, p.E, BM) * ((width + bno - 1) / bno);
+  const int grid = (int)std::min<int64_t>(tiles, cu_count() * (int)(kMaxLds / shm));
+  // whole pairs of steps, the first and the last apart; zeros past K
+  const int steps = std::max(4, 2 * ((p.K + 2 * kStep - 1) / (2 * kStep)));
+  const uint32_t abytes = (uint32_t)((int64_t)(p.M - 1) * p.lda + p.K);
+  const uint32_t bbytes = (uint32_t)((int64_t)(p.N - 1) * p.ldb + p.K);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), shm, st, p, abytes, bbytes, steps);
+  return hipGetLastError();
+}
+
+template <int WM, int QA, int QB>
+hipError_t launch_t(const Grouped& p, hipStream_t st) {
+  auto go = [&](auto od) {
+    constexpr int OD = decltype(od)::value;
+    if (p.silu)
+      return p.bias ? launch_k<WM, QA, QB, OD, true, true>(p, st) : launch_k<WM, QA, QB, OD, false, true>(p, st);
+    return p.bias ? launch_k<WM, QA, QB, OD, true, false>(p, st) : launch_k<WM, QA, QB, OD, false, false>(p, st);
+  };
+  if (p.out_dtype == I8L_BF16) return go(std::integral_constant<int, I8L_BF16>{});
+  if (p.out_dtype == I8L_F16) return go(std::integral_constant<int, I8L_F16>{});
+  return go(std::integral_constant<int, I8L_F32>{});
+}
+
+}  // namespace
+
+// Offsets of 32 bits with bit 31 to spare, 16-byte pieces of every row, whole vectors of the epilogue.
+bool grouped_phased_ok(const Grouped& p) {
+  const int es = elt_size(p.out_dtype);
+  const int64_t most = (int64_t)kOutside - 2 * kStep;   // (a step may be requested past K)
+  return p.K % 16 == 0 && aligned16(p.a) && aligned16(p.b) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
+         p.eb % 16 == 0 && p.N % (p.silu ? 16 : 8) == 0 && aligned16(p.sb) && aligned16(p.bias) &&
+         aligned16(p.out) && p.ldc * es % 16 == 0 && (int64_t)p.M * p.lda + 2 * p.K < most &&
+         (int64_t)p.N * p.ldb + 2 * p.K < most &&
+         (most_blocks(p.R, p.E, 64) + 1) * ((p.N + 63) / 64) < INT32_MAX / 4;
+}
+
+hipError_t launch_grouped_phased(int bm, const Grouped& p, hipStream_t st) {
+  if (bm == 64) return launch_t<1, 1, 1>(p, st);
+  if (bm == 128) return launch_t<2, 1, 2>(p, st);
+  return launch_t<2, 2, 2>(p, st);
+}
+
+}  // namespace i8l

@@ -151,17 +151,6 @@ __device__ __forceinline__ int select(const Route& r, int64_t t, int lane) {
 
 __device__ __forceinline__ int bucket(int32_t e, int E) { return e >= 0 && e < E ? e : E; }
 
-// Inclusive sum over the 64 lanes.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true);   // row_bcast 15, 31
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true);
-  return v;
-}
-
 struct OrderShared {
   int32_t count[kWaves][kMaxExperts + 1];   // of each wave's piece; then its next place
   int32_t before[kMaxExperts + 1];          // pairs of the expert in earlier runs

@@ -439,6 +439,138 @@ py::object qk_norm_rope(const at::Tensor& q, const at::Tensor& k,
   return py::make_tuple(qo, ko);
 }
 
+// The order's outputs: offsets [E + 1], tokens [T k], places [T, k], and the counts' workspace.
+struct Order {
+  at::Tensor offsets, tokens, places, ws;
+  int64_t ws_bytes;
+};
+Order order_outputs(const at::Tensor& like, int64_t T, int64_t E, int64_t k) {
+  Order o{empty_like_on(like, {E + 1}, at::kInt), empty_like_on(like, {T * k}, at::kInt),
+          empty_like_on(like, {T, k}, at::kInt), at::Tensor(),
+          i8l_moe_order_workspace_bytes(T, E, k)};
+  if (o.ws_bytes > 0) o.ws = empty_like_on(like, {o.ws_bytes / 4}, at::kInt);
+  return o;
+}
+
+py::object moe_route(const at::Tensor& x, int64_t k, const std::string& scoring, bool renormalize) {
+  if (x.dim() != 2 || !x.is_cuda() || loses_gradient(x)) return py::none();
+  const int32_t code = float_code(x.scalar_type());
+  const int64_t T = x.size(0), E = x.size(1);
+  const int scored = scoring == "softmax" ? 0 : scoring == "sigmoid" ? 1 : -1;
+  if (code < 0 || scored < 0 || T < 1 || k < 1 || k > E || (E > 1 && x.stride(1) != 1) ||
+      (T > 1 && x.stride(0) < E))
+    return py::none();
+  at::Tensor w = empty_like_on(x, {T, k}, at::kFloat), e = empty_like_on(x, {T, k}, at::kInt);
+  Order o = order_outputs(x, T, E, k);
+  const c10::DeviceGuard guard(x.device());
+  const int st = i8l_moe_route(
+      x.data_ptr(), row_stride(x), code, T, E, k, scored, renormalize ? 1 : 0, (float*)w.data_ptr(),
+      (int32_t*)e.data_ptr(), (int32_t*)o.offsets.data_ptr(), (int32_t*)o.tokens.data_ptr(),
+      (int32_t*)o.places.data_ptr(), o.ws_bytes > 0 ? o.ws.data_ptr() : nullptr, o.ws_bytes,
+      stream_of(x));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::make_tuple(w, e, o.offsets, o.tokens, o.places);
+}
+
+py::object moe_order(const at::Tensor& e, int64_t E) {
+  if (e.scalar_type() != at::kInt || e.dim() != 2 || !e.is_cuda() || !e.is_contiguous() || E < 1 ||
+      e.size(0) < 1 || e.size(1) < 1)
+    return py::none();
+  const int64_t T = e.size(0), k = e.size(1);
+  Order o = order_outputs(e, T, E, k);
+  const c10::DeviceGuard guard(e.device());
+  const int st = i8l_moe_order((const int32_t*)e.data_ptr(), T, E, k, (int32_t*)o.offsets.data_ptr(),
+                               (int32_t*)o.tokens.data_ptr(), (int32_t*)o.places.data_ptr(),
+                               o.ws_bytes > 0 ? o.ws.data_ptr() : nullptr, o.ws_bytes, stream_of(e));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::make_tuple(o.offsets, o.tokens, o.places);
+}
+
+py::object w8a8_grouped_mm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& sa,
+                           const at::Tensor& sb, const at::Tensor& offsets,
+                           at::ScalarType out_dtype, const c10::optional<at::Tensor>& bias,
+                           const c10::optional<at::Tensor>& rows,
+                           const c10::optional<at::Tensor>& out, bool silu) {
+  const int32_t out_code = float_code(out_dtype);
+  if (out_code < 0 || a.scalar_type() != at::kChar || b.scalar_type() != at::kChar ||
+      !a.is_cuda() || a.dim() != 2 || b.dim() != 3 || a.size(1) != b.size(1) || loses_gradient(sa) ||
+      loses_gradient(sb) || loses_gradient(bias) || loses_gradient(out))
+    return py::none();
+  const at::Device dev = a.device();
+  const int64_t M = a.size(0), K = a.size(1), E = b.size(0), N = b.size(2);
+  if (!M || !K || !E || !N || (silu && N % 2) || a.stride(1) != 1 || b.stride(1) != 1 ||
+      b.device() != dev || !plain_vector(sa, at::kFloat, dev) || !plain_vector(sb, at::kFloat, dev) ||
+      !plain_vector(offsets, at::kInt, dev) || offsets.dim() != 1 || offsets.size(0) != E + 1)
+    return py::none();
+  // scale_a [M], [M, 1] or one value of those shapes; scale_b [E, N] or [E, N, 1]
+  if (sa.dim() < 1 || sa.dim() > 2 || (sa.dim() == 2 && sa.size(1) != 1) ||
+      (sa.size(0) != M && sa.size(0) != 1) || sb.dim() < 2 || sb.dim() > 3 || sb.size(0) != E ||
+      sb.size(1) != N || (sb.dim() == 3 && sb.size(2) != 1))
+    return py::none();
+  int32_t bias_code = I8L_DTYPE_NONE;
+  if (bias.has_value()) {
+    bias_code = float_code(bias->scalar_type());
+    if (bias_code < 0 || bias->dim() != 2 || bias->size(0) != E || bias->size(1) != N ||
+        bias->device() != dev || !bias->is_contiguous())
+      return py::none();
+  }
+  if (rows.has_value() && (!plain_vector(*rows, at::kInt, dev) || rows->dim() != 1))
+    return py::none();
+  const int64_t R = rows.has_value() ? rows->size(0) : M, width = silu ? N / 2 : N;
+  at::Tensor o;
+  if (out.has_value()) {
+    o = *out;
+    if (o.dim() != 2 || o.size(0) != R || o.size(1) != width || o.scalar_type() != out_dtype ||
+        o.device() != dev || (width > 1 && o.stride(1) != 1) || (R > 1 && o.stride(0) < width))
+      return py::none();
+  } else {
+    o = empty_like_on(a, {R, width}, out_dtype);
+  }
+  const c10::DeviceGuard guard(dev);
+  const int st = i8l_w8a8_grouped_mm(
+      (const int8_t*)a.data_ptr(), row_stride(a), M,
+      rows.has_value() ? (const int32_t*)rows->data_ptr() : nullptr, (const int8_t*)b.data_ptr(),
+      b.stride(0), N > 1 ? b.stride(2) : K, (const float*)sa.data_ptr(), sa.numel(),
+      (const float*)sb.data_ptr(), bias.has_value() ? bias->data_ptr() : nullptr, bias_code,
+      (const int32_t*)offsets.data_ptr(), o.data_ptr(), row_stride(o), out_code, silu ? 1 : 0, R, E,
+      N, K, stream_of(a));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::cast(o);
+}
+
+py::object moe_combine(const at::Tensor& y, const at::Tensor& w, const at::Tensor& places,
+                       const c10::optional<at::Tensor>& base) {
+  const int32_t code = float_code(y.scalar_type());
+  if (code < 0 || !y.is_cuda() || y.dim() != 2 || places.dim() != 2 || w.dim() != 2 ||
+      loses_gradient(y) || loses_gradient(w) || loses_gradient(base))
+    return py::none();
+  const at::Device dev = y.device();
+  const int64_t T = places.size(0), k = places.size(1), R = y.size(0), N = y.size(1);
+  auto spaced = [&](const at::Tensor& t) {
+    return (N <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= N);
+  };
+  if (k < 1 || w.size(0) != T || w.size(1) != k || !plain_vector(w, at::kFloat, dev) ||
+      !plain_vector(places, at::kInt, dev) || !spaced(y))
+    return py::none();
+  if (base.has_value() &&
+      (base->scalar_type() != y.scalar_type() || base->dim() != 2 || base->size(0) != T ||
+       base->size(1) != N || base->device() != dev || !spaced(*base)))
+    return py::none();
+  at::Tensor out = empty_like_on(y, {T, N}, y.scalar_type());
+  const c10::DeviceGuard guard(dev);
+  const int st = i8l_moe_combine(y.data_ptr(), row_stride(y), R, (const float*)w.data_ptr(),
+                                 (const int32_t*)places.data_ptr(),
+                                 base.has_value() ? base->data_ptr() : nullptr,
+                                 base.has_value() ? row_stride(*base) : N, out.data_ptr(), T, k, N,
+                                 code, stream_of(y));
+  if (st != I8L_OK) return py::none();
+  ++g_launches;
+  return py::cast(out);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_i8l_fast, m) {
@@ -459,4 +591,8 @@ PYBIND11_MODULE(_i8l_fast, m) {
   m.def("silu_mul_mxfp4_quant", &silu_mul_mxfp4_quant);
   m.def("mxfp4_mm", &mxfp4_mm);
   m.def("qk_norm_rope", &qk_norm_rope);
+  m.def("moe_route", &moe_route);
+  m.def("moe_order", &moe_order);
+  m.def("w8a8_grouped_mm", &w8a8_grouped_mm);
+  m.def("moe_combine", &moe_combine);
 }

@@ -521,3 +521,43 @@ def test_custom_ops_run():
     h = ops.w8a8_grouped_mm_silu_mul(*args, torch.bfloat16, None, r.tokens)
     assert torch.equal(h, moe.w8a8_grouped_mm_silu_mul(*args, rows=r.tokens))
     assert torch.equal(ops.moe_combine(y, r.weights, r.places, None), moe.moe_combine(y, r.weights, r.places))
+
+
+# ------------------------------------------------------------------ the C++ binding
+def test_the_binding_takes_plain_calls_and_gives_the_same(monkeypatch):
+    from int8_linear import _lib
+    f = _lib.fast()
+    assert f is not None
+    logits = randn((9, 12), 2, 2.0)
+    p = problem([4] * 12, 64, 32, tokens=9)
+    bias = randn((12, 32), 3)
+    base = randn((9, 32), 4)
+
+    def calls():
+        r = moe.moe_route(logits, 3, scoring="sigmoid", renormalize=False)
+        args = (p["a"], p["w"].transpose(1, 2), p["sa"], p["sb"], r.offsets)
+        y = moe.w8a8_grouped_mm(*args, torch.float16, bias, rows=r.tokens)
+        h = moe.w8a8_grouped_mm_silu_mul(*args, rows=r.tokens, out=torch.zeros(27, 16, dtype=torch.bfloat16, device="cuda"))
+        z = moe.moe_combine(y, r.weights, r.places, base=base.half())
+        return [*r, *moe.moe_order(r.experts, 10), y, h, z]
+    before = f.launches()
+    fast = calls()
+    assert f.launches() == before + 5
+    monkeypatch.setattr("int8_linear.moe._fast", lambda *a: None)
+    slow = calls()
+    assert f.launches() == before + 5
+    for a, b in zip(fast, slow):
+        assert torch.equal(a, b)
+
+
+def test_the_binding_declines_a_lost_gradient():
+    p = problem([4, 4], 64, 32)
+    for name in ("sa", "sb"):
+        args = dict(p, **{name: p[name].clone().requires_grad_()})
+        with pytest.raises(NotSupported, match="no gradient"):
+            moe.w8a8_grouped_mm(args["a"], args["w"].transpose(1, 2), args["sa"], args["sb"], args["offsets"])
+    with pytest.raises(NotSupported, match="no gradient"):
+        moe.moe_route(torch.zeros(2, 4, device="cuda", requires_grad=True), 2)
+    y = torch.zeros(4, 8, device="cuda", requires_grad=True)
+    with pytest.raises(NotSupported, match="no gradient"):
+        moe.moe_combine(y, torch.zeros(2, 2, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda"))
