@@ -463,8 +463,8 @@ int64_t i8l_moe_order_workspace_bytes(int64_t T, int64_t E, int64_t k);
  * scale_a M values or one, scale_b and bias (bf16/f16/f32, or NULL) [E,N] contiguous; out [R,N] of
  * out_dtype (bf16/f16/f32), rows ldc elements apart.  With silu_mul the first N/2 columns are gate
  * values g, the others up values u, and out [R,N/2] = cast(g / (1 + exp(-g)) * u), all in fp32.
- * Rows from offsets[E] on are left as they were.  Offsets are held within [0,R] (rows
- * that none or several name hold anything); an r outside [0,M) gives NaN.  E up to 512, R up to 2^25, K below 2^17.  Any alignment;
+ * Rows from offsets[E] on are left as they were.  Offsets are held within [0,R], each to
+ * those before it; an r outside [0,M) gives NaN.  E up to 512, R up to 2^25, K below 2^17.  Any alignment;
  * fast where K, lda, ldb and expert_stride are multiples of 16, N of 8, and a, b, scale_b, bias and
  * out and its rows start on 16 bytes.  Nothing is allocated.
  */

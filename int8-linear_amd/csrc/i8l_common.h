@@ -210,6 +210,16 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
+// Inclusive maximum over the 64 lanes of values that are not negative.
+__device__ __forceinline__ int wave_max_scan(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, true));
+  return max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, true));
+}
+
 // Maximum over each aligned group of G lanes (G = 16, 32 or 64); every lane returns its
 // group's.  Four DPP steps cover a 16-lane row; a swizzle and a permute cover 32 and 64.
 template <int G>

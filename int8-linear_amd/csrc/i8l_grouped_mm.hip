@@ -95,13 +95,41 @@ hipError_t launch_any_v(const Grouped& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// The rows of a macro tile, by the rows an expert has on average.
-int phased_rows(int64_t R, int64_t E) {
-  const int64_t each = R / E;
-  return each <= 48 ? 64 : each <= 512 ? 128 : 256;
+// The rows of a tile by the rows that an expert has on average (their spread is not known here), where
+// one is faster than the next in us, over 2048 -> 1536 and 768 -> 2048 (128 experts), 2048 -> 2816 (60)
+// and 4096 -> 28672 (8), random choices, cold weights:
+//   ring 16 / 32        at 4 rows 55.1 / 57.9, 39.8 / 37.4, 45.1 / 47.2, 146 / 146; at 8 60.7 / 60.2,
+//                       44.5 / 40.8, 51.5 / 51.7, 157 / 150
+//   ring 32 / 64        at 8 60.2 / 64.4, 40.8 / 44.3, 51.7 / 53.7, 150 / 150; at 16 73.2 / 74.8,
+//                       50.0 / 50.7, 63.7 / 66.3, 165 / 157
+//   ring 64 / tile 64   at 16 74.8 / 77.1, 50.7 / 43.9, 66.3 / 68.6, 157 / 202; at 24 87.4 / 87.1,
+//                       57.9 / 50.1, 73.5 / 69.4, 167 / 205; at 48 110 / 94.6, 73.4 / 54.7, 90.0 / 76.6,
+//                       208 / 206: the ring streams the weights of a long K faster
+//   tile 64 / 128       at 48 94.6 / 95.4, 54.7 / 58.7, 76.6 / 74.6, 206 / 211; at 64 93.2 / 92.9,
+//                       61.0 / 60.4, 86.9 / 86.1, 209 / 214; at 96 114 / 100, 71.1 / 72.4, 98.2 / 92.5,
+//                       237 / 218
+//   tile 128 / 256      at 128 116 / 131, 79.1 / 85.2, 94.0 / 101, 242 / 245; at 256 165 / 161,
+//                       109 / 114, 145 / 149, 315 / 317; at 512 264 / 245, 176 / 173, 226 / 216, 523 / 517
+hipError_t launch_fast(const Grouped& p, hipStream_t st) {
+  const int64_t each = p.R / p.E;
+  if (each < 6) return launch_grouped_ring(16, p, st);
+  if (each < 14) return launch_grouped_ring(32, p, st);
+  if (each < (p.K >= 4096 ? 44 : p.K > 1024 ? 20 : 14)) return launch_grouped_ring(64, p, st);
+  return launch_grouped_phased(each < 64 ? 64 : each < 256 ? 128 : 256, p, st);
 }
 
 }  // namespace
+
+// Offsets of 32 bits with bit 31 to spare, 16-byte pieces of every row, whole vectors of the epilogue.
+bool grouped_fast_ok(const Grouped& p) {
+  const int es = elt_size(p.out_dtype);
+  const int64_t most = (int64_t)kOutside - 1024;   // (a step may be requested past K)
+  return p.K % 16 == 0 && aligned16(p.a) && aligned16(p.b) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
+         p.eb % 16 == 0 && p.N % (p.silu ? 16 : 8) == 0 && aligned16(p.sb) && aligned16(p.bias) &&
+         aligned16(p.out) && p.ldc * es % 16 == 0 && (int64_t)p.M * p.lda + 2 * p.K < most &&
+         (int64_t)p.N * p.ldb + 2 * p.K < most &&
+         (most_blocks(p.R, p.E, 16) + 1) * ((p.N + 31) / 32) < (1 << 22);
+}
 
 hipError_t launch_grouped_any(const Grouped& p, hipStream_t st) {
   const uint64_t bits = (uintptr_t)p.a | (uintptr_t)p.b | (uint64_t)p.lda | (uint64_t)p.eb |
@@ -162,7 +190,6 @@ extern "C" int i8l_w8a8_grouped_mm(const int8_t* a, int64_t lda, int64_t M, cons
   p.sa_per_row = scale_a_len != 1, p.bias_dtype = bias ? bias_dtype : I8L_DTYPE_NONE;
   p.out_dtype = out_dtype, p.silu = silu_mul != 0;
   const hipStream_t st = (hipStream_t)stream;
-  const hipError_t e = grouped_phased_ok(p) ? launch_grouped_phased(phased_rows(R, E), p, st)
-                                            : launch_grouped_any(p, st);
+  const hipError_t e = grouped_fast_ok(p) ? launch_fast(p, st) : launch_grouped_any(p, st);
   return hip_status(e, "w8a8_grouped_mm launch");
 }

@@ -31,53 +31,10 @@ namespace {
 // source rows of three tiles (read an epilogue ahead, where nothing but stores is in flight, so that
 // no wait for them drains the copies).
 //
-// The copies are buffer loads with the row's byte offset in a register and the K position in a scalar:
-// an offset past the buffer's size reads as zeros, which gives rows past the expert's last, whole
-// steps past K and its tail within a step their zeros at the price of one instruction a copy (zeros
-// toggle nothing: they cost little of the power that bounds the multiplications).
+// Rows past the expert's last, whole steps past K and its tail within a step are read outside the
+// buffers, as zeros, at the price of one instruction a copy (zeros toggle nothing: they cost little of
+// the power that bounds the multiplications).
 constexpr int kStep = 128;
-constexpr uint32_t kOutside = 0x80000000u;   // (the buffers are smaller than 2^31 bytes)
-
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-
-// A buffer of `bytes` bytes from p on, checked byte by byte (raw, no stride).
-__device__ __forceinline__ v4u buffer_of(const void* p, uint32_t bytes) {
-  const uint64_t a = (uint64_t)(uintptr_t)p;
-  return v4u{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a),
-             (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)) & 0xffffu,
-             (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), 0x00020000u};
-}
-
-// 16 bytes a lane into 1 KiB of LDS from `dst` on.  Assembly, so that the compiler, which cannot count
-// these among other requests, places no wait of its own: the phases' explicit waits cover them.
-__device__ __forceinline__ void copy_1k(v4u buf, uint32_t off, int at, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
-               ::"v"(off), "s"(buf), "s"(at), "s"(dst) : "memory", "m0");
-}
-
-// The scales and bias of 4 neighbouring columns of an expert (past the last: the last four's).
-struct ColQuad {
-  float sb[4], bias[4];
-};
-template <bool BIAS>
-__device__ __forceinline__ ColQuad load_quad(const Grouped& p, int64_t at, int n) {
-  n = min(n, p.N - 4);
-  ColQuad c;
-  const float4 s = *(const float4*)(p.sb + at + n);
-  c.sb[0] = s.x, c.sb[1] = s.y, c.sb[2] = s.z, c.sb[3] = s.w;
-  if constexpr (BIAS) {
-    if (p.bias_dtype == I8L_F32) {
-      const float4 b = *(const float4*)((const float*)p.bias + at + n);
-      c.bias[0] = b.x, c.bias[1] = b.y, c.bias[2] = b.z, c.bias[3] = b.w;
-    } else {
-      const uint2 h = *(const uint2*)((const uint16_t*)p.bias + at + n);
-      const uint32_t w[4] = {h.x & 0xffffu, h.x >> 16, h.y & 0xffffu, h.y >> 16};
-#pragma unroll
-      for (int r = 0; r < 4; ++r) c.bias[r] = act_to_f32(w[r], p.bias_dtype);
-    }
-  }
-  return c;
-}
 
 struct PhasedShared {
   int32_t first[kMaxExperts + 1];            // an expert's first block; [E]: their number
@@ -112,19 +69,18 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
 
   // ---- the experts' blocks
   if (wave == 0) {
-    const int per = (p.E + 63) / 64, e0 = min(lane * per, p.E), e1 = min(e0 + per, p.E);
-    int blocks = 0;
-    for (int e = e0; e < e1; ++e) {
-      int lo, hi;
-      expert_rows(p, e, lo, hi);
-      sh.lo[e] = lo;
-      sh.hi[e] = hi;
-      sh.first[e] = blocks;
-      blocks += (hi - lo + BM - 1) / BM;
+    int lowest = 0, before = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 64) {
+      const int e = min(e0 + lane, p.E - 1);
+      const bool in = e0 + lane < p.E;
+      const ExpertRows x = expert_rows(p, BM, in, p.offsets[e], p.offsets[e + 1], lowest, before);
+      if (in) {
+        sh.lo[e] = x.lo;
+        sh.hi[e] = x.hi;
+        sh.first[e] = x.upto - x.blocks;
+      }
     }
-    const int upto = wave_scan(blocks);
-    for (int e = e0; e < e1; ++e) sh.first[e] += upto - blocks;
-    if (lane == 63) sh.first[p.E] = upto;
+    if (lane == 0) sh.first[p.E] = before;
   }
   __syncthreads();
   const int total_blocks = __builtin_amdgcn_readfirstlane(sh.first[p.E]);
@@ -392,13 +348,6 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
           cl[c][q] = load_quad<BIAS>(p, ecol, SILU ? min(n, width - 4) : n);
           if constexpr (SILU) cu[c][q] = load_quad<BIAS>(p, ecol, width + min(n, width - 4));
         }
-      auto scaled = [&](int32_t a, float sa, const ColQuad& c, int r) {
-        float v = (float)a;
-        v = v * sa;
-        v = v * c.sb[r];
-        if constexpr (BIAS) v = v + c.bias[r];
-        return v;
-      };
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -414,10 +363,10 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
               for (int r = 0; r < 4; ++r) {
                 if constexpr (SILU) {
                   v[r] = silu_mul<OD == I8L_F32>(
-                      scaled(acc[h][0][i][x][4 * q + r], sam[h][i], cl[c][q], r),
-                      scaled(acc[h][1][i][x][4 * q + r], sam[h][i], cu[c][q], r));
+                      quad_value<BIAS>(acc[h][0][i][x][4 * q + r], sam[h][i], cl[c][q], r),
+                      quad_value<BIAS>(acc[h][1][i][x][4 * q + r], sam[h][i], cu[c][q], r));
                 } else {
-                  v[r] = scaled(acc[h][x / QB][i][x % QB][4 * q + r], sam[h][i], cl[c][q], r);
+                  v[r] = quad_value<BIAS>(acc[h][x / QB][i][x % QB][4 * q + r], sam[h][i], cl[c][q], r);
                 }
                 // the value itself is rounded to fp16 in a cast of its own: opaque, or the product
                 // and the cast become one v_fma_mixlo_f16, which rounds once
@@ -489,17 +438,6 @@ hipError_t launch_t(const Grouped& p, hipStream_t st) {
 }
 
 }  // namespace
-
-// Offsets of 32 bits with bit 31 to spare, 16-byte pieces of every row, whole vectors of the epilogue.
-bool grouped_phased_ok(const Grouped& p) {
-  const int es = elt_size(p.out_dtype);
-  const int64_t most = (int64_t)kOutside - 2 * kStep;   // (a step may be requested past K)
-  return p.K % 16 == 0 && aligned16(p.a) && aligned16(p.b) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
-         p.eb % 16 == 0 && p.N % (p.silu ? 16 : 8) == 0 && aligned16(p.sb) && aligned16(p.bias) &&
-         aligned16(p.out) && p.ldc * es % 16 == 0 && (int64_t)p.M * p.lda + 2 * p.K < most &&
-         (int64_t)p.N * p.ldb + 2 * p.K < most &&
-         (most_blocks(p.R, p.E, 64) + 1) * ((p.N + 63) / 64) < INT32_MAX / 4;
-}
 
 hipError_t launch_grouped_phased(int bm, const Grouped& p, hipStream_t st) {
   if (bm == 64) return launch_t<1, 1, 1>(p, st);

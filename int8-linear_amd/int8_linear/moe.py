@@ -213,8 +213,8 @@ def w8a8_grouped_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor,
     e's rows are offsets[e] to offsets[e + 1] - 1 (int32 [E + 1]); row i reads a_q[rows[i]] with its
     scale, or a_q[i] without rows.  The arithmetic is w8a8_mm's, bit for bit.  `out` [R, N] (unit
     column stride) takes the result; rows from offsets[E] on are left as they were there, and in a
-    new output hold anything.  A row outside a_q gives NaN; offsets are held within [0, R], and rows
-    that none or several of them name hold anything.  There is no backward: scales, a bias or an out that require a gradient are refused
+    new output hold anything.  A row outside a_q gives NaN; an offset outside [0, R] or below an earlier
+    one is held to those.  There is no backward: scales, a bias or an out that require a gradient are refused
     where gradients are recorded.
     """
     o = _grouped("w8a8_grouped_mm", False, a_q, b_q, scale_a, scale_b, offsets, out_dtype, bias, rows, out)
