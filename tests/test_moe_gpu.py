@@ -561,3 +561,42 @@ def test_the_binding_declines_a_lost_gradient():
     y = torch.zeros(4, 8, device="cuda", requires_grad=True)
     with pytest.raises(NotSupported, match="no gradient"):
         moe.moe_combine(y, torch.zeros(2, 2, device="cuda"), torch.zeros(2, 2, dtype=torch.int32, device="cuda"))
+
+
+# ------------------------------------------------------------------ every schedule
+@pytest.mark.parametrize("each", [1, 5, 6, 13, 14, 19, 20, 40, 63, 64, 200, 256])
+@pytest.mark.parametrize("k,n", [(128, 64), (144, 80), (896, 96), (1024, 272), (1040, 48), (1920, 320), (4112, 160)])
+def test_mm_at_the_borders_of_the_schedules(each, k, n):
+    """Each schedule at a K of whole and broken steps, shorter and longer than what it holds ahead."""
+    spread = [max(0, each + d) for d in (-3, 0, 4, -each, 0, each - 1)]
+    p = problem(spread + [6 * each - sum(spread)] if sum(spread) < 6 * each else spread, k, n, tokens=33)
+    check_mm(p)
+    check_mm(p, torch.float16, randn((p["w"].shape[0], n), 1, 1.0, torch.float16))
+    check_mm(p, silu=True)
+    check_mm(p, torch.float32, silu=True)
+
+
+def test_mm_operands_far_apart():
+    """Offsets past 32 bits: rows of A, experts, rows of the output."""
+    k, n = 256, 64
+    p = problem([3, 20, 70], k, n, tokens=3)
+    far = torch.zeros(2 * 1_100_000_000 + k, dtype=torch.int8, device="cuda")
+    a = far.as_strided((3, k), (1_100_000_000, 1))
+    a.copy_(p["a"])
+    q = dict(p, a=a)
+    check_mm(q)
+    check_mm(q, silu=True)
+    w = torch.zeros(2 * 1_100_000_000 + n * k, dtype=torch.int8, device="cuda").as_strided(
+        (3, n, k), (1_100_000_000, k, 1))
+    w.copy_(p["w"])
+    check_mm(dict(p, w=w))
+    del far, w, a, q
+    out = torch.zeros(92 * 50_000_000 + n, dtype=torch.bfloat16, device="cuda").as_strided((93, n), (50_000_000, 1))
+    check_mm(p, out=out)
+
+
+def test_combine_rows_far_apart():
+    y = torch.zeros(3 * 1_200_000_000 + 64, dtype=torch.bfloat16, device="cuda").as_strided((4, 64), (1_200_000_000, 1))
+    y.copy_(randn((4, 64), 1))
+    w = torch.rand(5, 2, device="cuda")
+    check_combine(y, w, places_of(5, 2, 4, 1))
