@@ -8,16 +8,18 @@
 //   order      a stable counting sort of the pairs' flat index t * k + j by expert; pairs of no
 //              expert (anything outside [0, E)) come last and are given place -1
 //
-// Selecting: a wave a token, lane l holding the experts l, l + 64, ...  The logits become unsigned
-// keys in the same order, so a pick is one maximum over the wave (DPP) and a compare of every
-// register against it, whose first set lane is the lowest expert; all of that is uniform.
+// Selecting: 16 lanes a token, four tokens a wave, lane l holding the experts l * C .. l * C + C - 1 (one
+// wide load).  The logits become unsigned keys in the same order; a pick is the largest key of the
+// lanes (DPP within their row of 16), then the smallest expert that has it
+// (which a 16-bit logit's key names itself).
 //
-// Ordering: up to kOneGroup pairs in one workgroup and one launch.  More are cut into up to kChunks
-// runs of tokens, one workgroup each: the first kernel selects and counts its run's pairs per
-// expert, the second one adds up the runs before its own (kChunks * E counts, from L2) and writes.
-// Within a run the waves take consecutive pieces, counted by LDS adds (sums of ones: any order) and
-// then walked 64 pairs at a time, a pair's rank among equals from ballots of the expert's bits.  No
-// atomic decides an order, so a call's results are the same every time.
+// Ordering: up to 64 pairs by one wave, whose lanes compare their experts bit by bit with ballots; up
+// to kOneGroup pairs in one workgroup and one launch.  More are cut into up to kChunks runs of tokens,
+// one workgroup each: the first kernel selects and counts its run's pairs per expert, the second one
+// adds up the runs before its own (all counts, from L2) and writes.  Within a run the waves take
+// consecutive pieces, counted by LDS adds (sums of ones: any order) and then walked 64 pairs at a time,
+// a pair's rank among equals from ballots of the expert's bits.  No atomic decides an order, so a call's
+// results are the same every time.
 #include "i8l_common.h"
 
 #include <algorithm>
@@ -28,58 +30,94 @@ namespace {
 
 constexpr int kWaves = 16, kThreads = 64 * kWaves;
 constexpr int kMaxExperts = 512, kMaxPicks = 64;
+constexpr int kSmall = 64;            // pairs that one wave orders
 constexpr int64_t kOneGroup = 1024;   // pairs that one workgroup orders in the selecting launch
-constexpr int kChunks = 128;          // runs of tokens otherwise
-constexpr int kMinRun = 32;           // tokens of a run at least
+constexpr int kChunks = 256;          // runs of tokens otherwise
+constexpr int kMinRun = 4 * kWaves;   // tokens of a run at least: a round of the selecting waves
 
 struct Route {
   const void* logits;       // NULL: `experts` are given
   int64_t ldl;
   float* weights;
   int32_t *experts, *offsets, *tokens, *places;
-  int32_t* counts;          // [chunks][E + 1]
+  int32_t* counts;          // [chunks][count_pitch(E)]
   int T, E, k, run, chunks; // run: tokens of a chunk
   int dtype, sigmoid, renormalize;
 };
 
-__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-  v = max(v, (uint32_t)dpp_i<kQuadSwap1>((int)v));
-  v = max(v, (uint32_t)dpp_i<kQuadSwap2>((int)v));
-  v = max(v, (uint32_t)dpp_i<kHalfMirror>((int)v));
-  v = max(v, (uint32_t)dpp_i<kRowMirror>((int)v));
-  const uint32_t a = max((uint32_t)__builtin_amdgcn_readlane((int)v, 0),
-                         (uint32_t)__builtin_amdgcn_readlane((int)v, 16));
-  const uint32_t b = max((uint32_t)__builtin_amdgcn_readlane((int)v, 32),
-                         (uint32_t)__builtin_amdgcn_readlane((int)v, 48));
-  return max(a, b);
+// Runs' counts are read four experts at a time.
+__host__ __device__ constexpr int count_pitch(int E) { return (E + 1 + 3) & ~3; }
+
+// Reductions over the 16 lanes of a DPP row; every lane returns its row's.
+template <typename F>
+__device__ __forceinline__ uint32_t row_reduce(uint32_t v, F f) {
+  v = f(v, (uint32_t)dpp_i<kQuadSwap1>((int)v));
+  v = f(v, (uint32_t)dpp_i<kQuadSwap2>((int)v));
+  v = f(v, (uint32_t)dpp_i<kHalfMirror>((int)v));
+  return f(v, (uint32_t)dpp_i<kRowMirror>((int)v));
+}
+__device__ __forceinline__ uint32_t row_umax(uint32_t v) {
+  return row_reduce(v, [](uint32_t a, uint32_t b) { return max(a, b); });
+}
+__device__ __forceinline__ uint32_t row_umin(uint32_t v) {
+  return row_reduce(v, [](uint32_t a, uint32_t b) { return min(a, b); });
+}
+__device__ __forceinline__ float row_sum(float v) {
+  return __uint_as_float(row_reduce(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
-  v = v + __int_as_float(dpp_i<kQuadSwap1>(__float_as_int(v)));
-  v = v + __int_as_float(dpp_i<kQuadSwap2>(__float_as_int(v)));
-  v = v + __int_as_float(dpp_i<kHalfMirror>(__float_as_int(v)));
-  v = v + __int_as_float(dpp_i<kRowMirror>(__float_as_int(v)));
-  float s[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    s[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16 * i));
-  return (s[0] + s[1]) + (s[2] + s[3]);
-}
-
-// Keys in the order of the floats, never 0 for a number; 0 for -inf and NaN.  (-0 counts as 0.)
-__device__ __forceinline__ uint32_t key_of(float x) {
-  const uint32_t b = __float_as_uint(x + 0.0f);
-  const uint32_t u = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-  return x > -__builtin_inff() ? u : 0u;
-}
-__device__ __forceinline__ float of_key(uint32_t u) {
-  return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u);
-}
-
+// Keys in the order of the logits, 0 for -inf and NaN only; -0 counts as 0.  A 16-bit logit's key holds
+// the expert too, the lower the larger, so that keys differ and the largest names its expert.
 template <int DT>
-__device__ __forceinline__ float load_logit(const void* p, int64_t i) {
-  if constexpr (DT == I8L_F32) return ((const float*)p)[i];
-  else return act_to_f32<DT>(((const uint16_t*)p)[i]);
+__device__ __forceinline__ uint32_t key_of(uint32_t bits, int e) {
+  if constexpr (DT == I8L_F32) {
+    const float x = __uint_as_float(bits);
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return x > -__builtin_inff() ? b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u) : 0u;
+  } else {
+    constexpr uint32_t inf = DT == I8L_BF16 ? 0x7f80u : 0x7c00u;
+    const uint32_t b = bits == 0x8000u ? 0u : bits;
+    const uint32_t u = b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+    return (b & 0x7fffu) > inf || b == (inf | 0x8000u) ? 0u : u << 16 | (0xffffu - e);
+  }
+}
+template <int DT>
+__device__ __forceinline__ float of_key(uint32_t key) {
+  if constexpr (DT == I8L_F32)
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+  const uint32_t u = key >> 16;
+  return act_to_f32<DT == I8L_F32 ? I8L_BF16 : DT>(u & 0x8000u ? u & 0x7fffu : ~u & 0xffffu);
+}
+
+// Logits [e0, e0 + C) of a row of E as keys, 0 past the last.  VEC: 16-byte aligned rows of whole
+// vectors.
+template <int C, int DT, bool VEC>
+__device__ __forceinline__ void load_keys(const void* row, int e0, int E, uint32_t (&key)[C]) {
+  if constexpr (VEC) {
+    constexpr int V = DT == I8L_F32 ? 4 : 8;
+#pragma unroll
+    for (int c = 0; c < C; c += V) {
+      const bool in = e0 + c < E;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (in) v = *(const uint4*)((const char*)row + (int64_t)(e0 + c) * (DT == I8L_F32 ? 4 : 2));
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const uint32_t w = chunk_word(v, DT == I8L_F32 ? i : i / 2);
+        const uint32_t x = DT == I8L_F32 ? w : i % 2 ? w >> 16 : w & 0xffffu;
+        key[c + i] = in ? key_of<DT>(x, e0 + c + i) : 0u;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      key[c] = 0;
+      if (e0 + c < E)
+        key[c] = key_of<DT>(DT == I8L_F32 ? ((const uint32_t*)row)[e0 + c] : ((const uint16_t*)row)[e0 + c],
+                            e0 + c);
+    }
+  }
 }
 
 // exp(x - top) of the pickable; equal ones (both +inf among them) give 1
@@ -91,80 +129,97 @@ __device__ __forceinline__ float sigmoid(float x) {
   return (x >= 0.0f ? 1.0f : z) / (1.0f + z);
 }
 
-// The picks of token t by one wave: lane j < k holds pick j's expert (-1: none).
-template <int C, int DT>
-__device__ __forceinline__ int select(const Route& r, int64_t t, int lane) {
-  uint32_t key[C];
+// The picks of the tokens t0 .. t0 + 3 by one wave, 16 lanes each: lane l of 16 holds pick 16 s + l's
+// expert in expert[s] (-1: none).  Tokens from t1 on: no picks, nothing written.
+constexpr int kSlots = kMaxPicks / 16;
+template <int C, int DT, bool VEC>
+__device__ __forceinline__ void select(const Route& r, int t0, int t1, int lane, int (&expert)[kSlots]) {
+  const int l = lane & 15, t = t0 + (lane >> 4);
+  const bool in = t < t1;
+  uint32_t key[C], mine[kSlots] = {};
+  load_keys<C, DT, VEC>((const char*)r.logits + (in ? t : t0) * r.ldl * (DT == I8L_F32 ? 4 : 2), l * C,
+                        r.E, key);
+  float total = 0.0f;
+  uint32_t top = key[0];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int e = 64 * c + lane;
-    key[c] = e < r.E ? key_of(load_logit<DT>(r.logits, t * r.ldl + e)) : 0u;
+  for (int c = 1; c < C; ++c) top = max(top, key[c]);
+  top = row_umax(top);
+  const float tx = of_key<DT>(top);
+  if (!r.renormalize && !r.sigmoid) {
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (key[c]) total += soft(of_key<DT>(key[c]), tx);
+    total = row_sum(total);
   }
-  uint32_t all[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) all[c] = key[c];
-  int expert = -1;
-  uint32_t mine = 0, top = 0;
-  for (int j = 0; j < r.k; ++j) {
-    uint32_t best = key[0];
+  for (int s = 0; s < kSlots; ++s) {
+    expert[s] = -1;
+    for (int j = 16 * s; j < min(r.k, 16 * s + 16); ++j) {
+      uint32_t best = key[0];
 #pragma unroll
-    for (int c = 1; c < C; ++c) best = max(best, key[c]);
-    best = wave_umax(best);
-    if (best == 0) break;   // nothing left to pick
-    if (j == 0) top = best;
-    int at = 0, first = 0;
+      for (int c = 1; c < C; ++c) best = max(best, key[c]);
+      best = row_umax(best);
+      uint32_t first = ~0u;
+      if constexpr (DT == I8L_F32) {
 #pragma unroll
-    for (int c = C - 1; c >= 0; --c) {
-      const uint64_t m = __ballot(key[c] == best);
-      if (m) at = c, first = __builtin_ctzll(m);
+        for (int c = C - 1; c >= 0; --c) first = key[c] == best ? l * C + c : first;
+        first = row_umin(first);
+#pragma unroll
+        for (int c = 0; c < C; ++c) key[c] = first == l * C + c ? 0u : key[c];
+      } else {
+        first = 0xffffu - (best & 0xffffu);
+#pragma unroll
+        for (int c = 0; c < C; ++c) key[c] = key[c] == best ? 0u : key[c];
+      }
+      // (with nothing left to pick, best is 0)
+      if (j == 16 * s + l && best) expert[s] = (int)first, mine[s] = best;
     }
+  }
+  float p[kSlots];
+  float picked = 0.0f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (c == at && lane == first) key[c] = 0;
-    if (lane == j) expert = 64 * at + first, mine = best;
+  for (int s = 0; s < kSlots; ++s) {
+    p[s] = 0.0f;
+    if (16 * s < r.k && expert[s] >= 0) {
+      const float x = of_key<DT>(mine[s]);
+      if (!r.sigmoid) p[s] = soft(x, tx);
+      else if (!r.renormalize || tx >= 0.0f) p[s] = sigmoid(x);
+      else p[s] = soft(x, tx) / (1.0f + canon_expf(x));   // over exp(max): the sum of any logits is not 0
+    }
+    picked += p[s];
   }
-  const float tx = of_key(top);
-  float p = 0.0f, total = 0.0f;
-  if (expert >= 0) {
-    const float x = of_key(mine);
-    if (!r.sigmoid) p = soft(x, tx);
-    else if (!r.renormalize || tx >= 0.0f) p = sigmoid(x);
-    else p = soft(x, tx) / (1.0f + canon_expf(x));   // over exp(max): the sum of any logits is not 0
-  }
-  if (r.renormalize) {
-    total = wave_sum(p);
-  } else if (!r.sigmoid) {
+  if (r.renormalize) total = row_sum(picked);
+  else if (r.sigmoid) total = 1.0f;
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-      if (all[c]) total += soft(of_key(all[c]), tx);
-    total = wave_sum(total);
-  } else {
-    total = 1.0f;
+  for (int s = 0; s < kSlots; ++s) {
+    if (!in) expert[s] = -1;
+    if (in && 16 * s + l < r.k) {
+      const int64_t at = (int64_t)t * r.k + 16 * s + l;
+      r.weights[at] = total > 0.0f ? p[s] / total : 0.0f;
+      r.experts[at] = expert[s];
+    }
   }
-  if (lane < r.k) {
-    const int64_t at = t * r.k + lane;
-    r.weights[at] = total > 0.0f ? p / total : 0.0f;
-    r.experts[at] = expert;
-  }
-  return expert;
 }
 
 __device__ __forceinline__ int bucket(int32_t e, int E) { return e >= 0 && e < E ? e : E; }
 
+template <int W>
 struct OrderShared {
-  int32_t count[kWaves][kMaxExperts + 1];   // of each wave's piece; then its next place
+  int32_t count[W][kMaxExperts + 1];       // of each wave's piece; then its next place
   int32_t before[kMaxExperts + 1];          // pairs of the expert in earlier runs
   int32_t total[kMaxExperts + 1];           // in all runs; then the expert's first place
 };
 
 // The order of one run, [t0, t1), whose experts are in memory.  counts: the runs' counts, or NULL
 // where the run is all there is.
-__device__ __forceinline__ void order_run(const Route& r, int chunk, int t0, int t1, OrderShared& sh) {
+template <int W>
+__device__ __forceinline__ void order_run(const Route& r, int chunk, int t0, int t1, OrderShared<W>& sh) {
+  constexpr int kThreads = 64 * W;
   const int lane = threadIdx.x & 63, tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int B = r.E + 1;
   const int i0 = t0 * r.k, n = (t1 - t0) * r.k;
-  const int piece = ((n + kWaves - 1) / kWaves + 63) & ~63;
+  const int piece = ((n + W - 1) / W + 63) & ~63;
   const int w0 = min(wave * piece, n), w1 = min(w0 + piece, n);
   for (int b = lane; b < B; b += 64) sh.count[wave][b] = 0;
   if (r.chunks > 1)
@@ -173,19 +228,24 @@ __device__ __forceinline__ void order_run(const Route& r, int chunk, int t0, int
   for (int i = w0 + lane; i < w1; i += 64)
     atomicAdd(&sh.count[wave][bucket(r.experts[i0 + i], r.E)], 1);
   if (r.chunks > 1) {
-    // the runs' counts, several threads an expert, each a share of the runs
-    const int share = max(1, kThreads / B);
-    for (int x = tid; x < share * B; x += kThreads) {
-      const int b = x % B;
-      int early = 0, all = 0;
+    // the runs' counts, four experts a thread and several threads for them, each a share of the runs
+    const int P = count_pitch(r.E) / 4, share = kThreads / P;
+    if (tid < share * P) {
+      const int b = tid % P * 4;
+      int4 early = make_int4(0, 0, 0, 0), all = early;
 #pragma unroll 8
-      for (int c = x / B; c < r.chunks; c += share) {
-        const int v = r.counts[c * B + b];
-        all += v;
-        early += c < chunk ? v : 0;
+      for (int c = tid / P; c < r.chunks; c += share) {
+        const int4 v = *(const int4*)(r.counts + (int64_t)c * (4 * P) + b);
+        all.x += v.x, all.y += v.y, all.z += v.z, all.w += v.w;
+        if (c < chunk) early.x += v.x, early.y += v.y, early.z += v.z, early.w += v.w;
       }
-      atomicAdd(&sh.before[b], early);
-      atomicAdd(&sh.total[b], all);
+      const int e[4] = {early.x, early.y, early.z, early.w}, a[4] = {all.x, all.y, all.z, all.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (b + i < B) {
+          atomicAdd(&sh.before[b + i], e[i]);
+          atomicAdd(&sh.total[b + i], a[i]);
+        }
     }
   }
   __syncthreads();
@@ -193,7 +253,7 @@ __device__ __forceinline__ void order_run(const Route& r, int chunk, int t0, int
     for (int b = tid; b < B; b += kThreads) {
       int v = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) v += sh.count[w][b];
+      for (int w = 0; w < W; ++w) v += sh.count[w][b];
       sh.total[b] = v;
       sh.before[b] = 0;
     }
@@ -214,7 +274,7 @@ __device__ __forceinline__ void order_run(const Route& r, int chunk, int t0, int
   for (int b = tid; b < B; b += kThreads) {
     int at = sh.total[b] + sh.before[b];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       const int v = sh.count[w][b];
       sh.count[w][b] = at;
       at += v;
@@ -244,25 +304,68 @@ __device__ __forceinline__ void order_run(const Route& r, int chunk, int t0, int
   }
 }
 
-template <int C, int DT>
-__device__ __forceinline__ void select_run(const Route& r, int t0, int t1) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  for (int t = t0 + wave; t < t1; t += kWaves) select<C, DT>(r, t, threadIdx.x & 63);
-}
-
-// The whole of a small call.  C = 0: experts are given.
-template <int C, int DT>
-__global__ void __launch_bounds__(kThreads) moe_route_one(Route r) {
-  __shared__ OrderShared sh;
+// Up to kSmall pairs.  C = 0: experts are given.
+template <int C, int DT, bool VEC>
+__global__ void __launch_bounds__(256) moe_route_small(Route r) {
+  __shared__ int32_t pair[kSmall], sorted[kSmall];
+  const int tid = threadIdx.x, lane = tid & 63, n = r.T * r.k;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   if constexpr (C > 0) {
-    select_run<C, DT>(r, 0, r.T);
+    for (int t0 = 4 * wave; t0 < r.T; t0 += 16) {
+      int expert[kSlots];
+      select<C, DT, VEC>(r, t0, r.T, lane, expert);
+      const int t = t0 + (lane >> 4);
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) {
+        const int j = 16 * s + (lane & 15);
+        if (t < r.T && j < r.k) pair[t * r.k + j] = expert[s];
+      }
+    }
+    __syncthreads();
+  }
+  if (wave == 0) {
+    const bool in = lane < n;
+    int b = 0x3ff;   // (past every expert: behind all)
+    if (in) b = bucket(C > 0 ? pair[lane] : r.experts[lane], r.E);
+    uint64_t less = 0, same = ~(uint64_t)0;
+    for (int x = 9; x >= 0; --x) {
+      const uint64_t m = __ballot((b >> x) & 1);
+      if ((b >> x) & 1) less |= same & ~m, same &= m;
+      else same &= ~m;
+    }
+    const int place = __popcll(less) + __popcll(same & (((uint64_t)1 << lane) - 1));
+    sorted[place] = b;
+    if (in) {
+      r.places[lane] = b < r.E ? place : -1;
+      r.tokens[place] = b < r.E ? lane / r.k : -1;
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e <= r.E; e += 256) {   // pairs of experts below e
+    int at = 0;
+#pragma unroll
+    for (int step = kSmall / 2; step; step /= 2)
+      if (sorted[at + step - 1] < e) at += step;
+    r.offsets[e] = at + (at == kSmall - 1 && sorted[at] < e);
+  }
+}
+static_assert(kMaxExperts < 0x3ff, "the bits of an expert");
+
+// The whole of a call of up to kOneGroup pairs.
+template <int C, int DT, bool VEC>
+__global__ void __launch_bounds__(kThreads) moe_route_one(Route r) {
+  __shared__ OrderShared<kWaves> sh;
+  if constexpr (C > 0) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int expert[kSlots];
+    for (int t = 4 * wave; t < r.T; t += 4 * kWaves) select<C, DT, VEC>(r, t, r.T, threadIdx.x & 63, expert);
     __syncthreads();   // the experts are in memory: order_run reads them from other waves
   }
   order_run(r, 0, 0, r.T, sh);
 }
 
 // A run's picks, and its pairs per expert.
-template <int C, int DT>
+template <int C, int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) moe_select(Route r) {
   __shared__ int32_t count[kMaxExperts + 1];
   const int t0 = blockIdx.x * r.run, t1 = min(t0 + r.run, r.T), lane = threadIdx.x & 63;
@@ -270,43 +373,59 @@ __global__ void __launch_bounds__(kThreads) moe_select(Route r) {
   __syncthreads();
   if constexpr (C > 0) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int t = t0 + wave; t < t1; t += kWaves) {
-      const int e = select<C, DT>(r, t, lane);
-      if (lane < r.k) atomicAdd(&count[bucket(e, r.E)], 1);
+    for (int t = t0 + 4 * wave; t < t1; t += 4 * kWaves) {
+      int expert[kSlots];
+      select<C, DT, VEC>(r, t, t1, lane, expert);
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s)
+        if (t + (lane >> 4) < t1 && 16 * s + (lane & 15) < r.k)
+          atomicAdd(&count[bucket(expert[s], r.E)], 1);
     }
   } else {
     for (int i = t0 * r.k + threadIdx.x; i < t1 * r.k; i += kThreads)
       atomicAdd(&count[bucket(r.experts[i], r.E)], 1);
   }
   __syncthreads();
-  for (int b = threadIdx.x; b <= r.E; b += kThreads)
-    r.counts[(int64_t)blockIdx.x * (r.E + 1) + b] = count[b];
+  const int P = count_pitch(r.E);
+  for (int b = threadIdx.x; b < P; b += kThreads)
+    r.counts[(int64_t)blockIdx.x * P + b] = b <= r.E ? count[b] : 0;
 }
 
-__global__ void __launch_bounds__(kThreads) moe_order(Route r) {
-  __shared__ OrderShared sh;
+// (eight waves: a run of 64 tokens of 8 picks is 64 pairs a wave)
+constexpr int kOrderWaves = 8;
+__global__ void __launch_bounds__(64 * kOrderWaves) moe_order(Route r) {
+  __shared__ OrderShared<kOrderWaves> sh;
   const int t0 = blockIdx.x * r.run;
   order_run(r, blockIdx.x, t0, min(t0 + r.run, r.T), sh);
 }
 
-template <int C, int DT>
+template <int C, int DT, bool VEC>
 hipError_t launch_route(const Route& r, hipStream_t st) {
-  if (r.chunks == 1) {
-    hipLaunchKernelGGL((moe_route_one<C, DT>), dim3(1), dim3(kThreads), 0, st, r);
+  if ((int64_t)r.T * r.k <= kSmall) {
+    hipLaunchKernelGGL((moe_route_small<C, DT, VEC>), dim3(1), dim3(256), 0, st, r);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL((moe_select<C, DT>), dim3(r.chunks), dim3(kThreads), 0, st, r);
+  if (r.chunks == 1) {
+    hipLaunchKernelGGL((moe_route_one<C, DT, VEC>), dim3(1), dim3(kThreads), 0, st, r);
+    return hipGetLastError();
+  }
+  hipLaunchKernelGGL((moe_select<C, DT, VEC>), dim3(r.chunks), dim3(kThreads), 0, st, r);
   if (const hipError_t e = hipGetLastError()) return e;
-  hipLaunchKernelGGL(moe_order, dim3(r.chunks), dim3(kThreads), 0, st, r);
+  hipLaunchKernelGGL(moe_order, dim3(r.chunks), dim3(64 * kOrderWaves), 0, st, r);
   return hipGetLastError();
 }
 
 template <int DT>
 hipError_t launch_route_dt(const Route& r, hipStream_t st) {
-  if (r.E <= 64) return launch_route<1, DT>(r, st);
-  if (r.E <= 128) return launch_route<2, DT>(r, st);
-  if (r.E <= 256) return launch_route<4, DT>(r, st);
-  return launch_route<8, DT>(r, st);
+  constexpr int V = DT == I8L_F32 ? 4 : 8;
+  const bool vec = ((uintptr_t)r.logits & 15) == 0 && r.ldl % V == 0 && r.E % V == 0;
+  auto go = [&](auto vc) {
+    constexpr bool VEC = decltype(vc)::value;
+    if (r.E <= 128) return launch_route<8, DT, VEC>(r, st);
+    if (r.E <= 256) return launch_route<16, DT, VEC>(r, st);
+    return launch_route<32, DT, VEC>(r, st);
+  };
+  return vec ? go(std::true_type{}) : go(std::false_type{});
 }
 
 // Tokens of a run and the number of runs.
@@ -337,14 +456,14 @@ int run_route(const char* who, Route r, int64_t T, int64_t E, int64_t k, void* w
   r.T = (int)T, r.E = (int)E, r.k = (int)k;
   plan_runs(T, k, &r.run, &r.chunks);
   const int64_t need = i8l_moe_order_workspace_bytes(T, E, k);
-  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3))) {
+  if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15))) {
     set_error("%s: a workspace of %lld bytes is needed, got %lld", who, (long long)need,
               (long long)(workspace ? workspace_bytes : 0));
     return I8L_INVALID_ARG;
   }
   r.counts = (int32_t*)workspace;
   hipError_t e;
-  if (!r.logits) e = launch_route<0, I8L_F32>(r, st);
+  if (!r.logits) e = launch_route<0, I8L_F32, false>(r, st);
   else if (r.dtype == I8L_BF16) e = launch_route_dt<I8L_BF16>(r, st);
   else if (r.dtype == I8L_F16) e = launch_route_dt<I8L_F16>(r, st);
   else e = launch_route_dt<I8L_F32>(r, st);
@@ -361,7 +480,7 @@ extern "C" int64_t i8l_moe_order_workspace_bytes(int64_t T, int64_t E, int64_t k
     return 0;
   int run, chunks;
   plan_runs(T, k, &run, &chunks);
-  return chunks > 1 ? (int64_t)chunks * (E + 1) * 4 : 0;
+  return chunks > 1 ? (int64_t)chunks * count_pitch((int)E) * 4 : 0;
 }
 
 extern "C" int i8l_moe_route(const void* logits, int64_t ldl, int32_t dtype, int64_t T, int64_t E,

@@ -25,7 +25,7 @@ orders its own with moe_order (any expert outside [0, n_experts) is elsewhere); 
 offsets[n_experts] on are then not computed, and moe_combine leaves those pairs out.
 
 Launches go on the caller's current stream and allocate nothing but the outputs and, for more than
-1024 pairs, the ordering's counts (up to 257 KiB).  There is no backward: what would carry a gradient
+1024 pairs, the ordering's counts (up to 516 KiB).  There is no backward: what would carry a gradient
 is refused where gradients are recorded.
 """
 
