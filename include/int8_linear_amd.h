@@ -443,8 +443,9 @@ int i8l_qk_norm_rope(const void* q, int64_t q_ts, int64_t q_hs, const void* k, i
  *   places [T,k]   the ordered row of each pair, -1 for a pair without an expert
  * Pairs of one expert keep their order (t, then choice).  E up to 512, k up to 64 and E, T*k up to
  * 2^25.  i8l_moe_order gives the order of experts picked elsewhere: any value outside [0,E) is a pair
- * without an expert here.  workspace: i8l_moe_order_workspace_bytes(T,E,k) bytes (0: none is needed),
- * 16-byte aligned, not shared by calls that overlap.
+ * without an expert here.  workspace: the bytes that i8l_moe_route_workspace_bytes and
+ * i8l_moe_order_workspace_bytes name (0: none is needed), 16-byte aligned, not shared by calls that
+ * overlap.
  */
 int i8l_moe_route(const void* logits, int64_t ldl, int32_t logits_dtype, int64_t T, int64_t E,
                   int64_t k, int32_t scoring, int32_t renormalize, float* weights, int32_t* experts,
@@ -453,6 +454,7 @@ int i8l_moe_route(const void* logits, int64_t ldl, int32_t logits_dtype, int64_t
 int i8l_moe_order(const int32_t* experts, int64_t T, int64_t E, int64_t k, int32_t* offsets,
                   int32_t* tokens, int32_t* places, void* workspace, int64_t workspace_bytes,
                   void* stream);
+int64_t i8l_moe_route_workspace_bytes(int64_t T, int64_t E, int64_t k);
 int64_t i8l_moe_order_workspace_bytes(int64_t T, int64_t E, int64_t k);
 
 /*

@@ -444,10 +444,9 @@ struct Order {
   at::Tensor offsets, tokens, places, ws;
   int64_t ws_bytes;
 };
-Order order_outputs(const at::Tensor& like, int64_t T, int64_t E, int64_t k) {
+Order order_outputs(const at::Tensor& like, int64_t T, int64_t E, int64_t k, int64_t ws_bytes) {
   Order o{empty_like_on(like, {E + 1}, at::kInt), empty_like_on(like, {T * k}, at::kInt),
-          empty_like_on(like, {T, k}, at::kInt), at::Tensor(),
-          i8l_moe_order_workspace_bytes(T, E, k)};
+          empty_like_on(like, {T, k}, at::kInt), at::Tensor(), ws_bytes};
   if (o.ws_bytes > 0) o.ws = empty_like_on(like, {o.ws_bytes / 4}, at::kInt);
   return o;
 }
@@ -461,7 +460,7 @@ py::object moe_route(const at::Tensor& x, int64_t k, const std::string& scoring,
       (T > 1 && x.stride(0) < E))
     return py::none();
   at::Tensor w = empty_like_on(x, {T, k}, at::kFloat), e = empty_like_on(x, {T, k}, at::kInt);
-  Order o = order_outputs(x, T, E, k);
+  Order o = order_outputs(x, T, E, k, i8l_moe_route_workspace_bytes(T, E, k));
   const c10::DeviceGuard guard(x.device());
   const int st = i8l_moe_route(
       x.data_ptr(), row_stride(x), code, T, E, k, scored, renormalize ? 1 : 0, (float*)w.data_ptr(),
@@ -478,7 +477,7 @@ py::object moe_order(const at::Tensor& e, int64_t E) {
       e.size(0) < 1 || e.size(1) < 1)
     return py::none();
   const int64_t T = e.size(0), k = e.size(1);
-  Order o = order_outputs(e, T, E, k);
+  Order o = order_outputs(e, T, E, k, i8l_moe_order_workspace_bytes(T, E, k));
   const c10::DeviceGuard guard(e.device());
   const int st = i8l_moe_order((const int32_t*)e.data_ptr(), T, E, k, (int32_t*)o.offsets.data_ptr(),
                                (int32_t*)o.tokens.data_ptr(), (int32_t*)o.places.data_ptr(),

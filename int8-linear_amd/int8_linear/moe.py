@@ -25,7 +25,7 @@ orders its own with moe_order (any expert outside [0, n_experts) is elsewhere); 
 offsets[n_experts] on are then not computed, and moe_combine leaves those pairs out.
 
 Launches go on the caller's current stream and allocate nothing but the outputs and, for more than
-1024 pairs, the ordering's counts (up to 516 KiB).  There is no backward: what would carry a gradient
+64 tokens, the ordering's counts (up to 516 KiB).  There is no backward: what would carry a gradient
 is refused where gradients are recorded.
 """
 
@@ -53,12 +53,11 @@ class Routing(NamedTuple):
     places: torch.Tensor    # int32 [T, k]: the row of each pair, -1 where it has no expert
 
 
-def _order_outputs(t: int, e: int, k: int, device: torch.device):
-    """The order's outputs and its workspace (None where none is needed)."""
+def _order_outputs(t: int, e: int, k: int, need: int, device: torch.device):
+    """The order's outputs and its workspace of `need` bytes (None of 0)."""
     def ints(*shape):
         return torch.empty(shape, dtype=torch.int32, device=device)
-    need = _lib.lib().i8l_moe_order_workspace_bytes(t, e, k)
-    return ints(e + 1), ints(t * k), ints(t, k), ints(need // 4) if need else None, need
+    return ints(e + 1), ints(t * k), ints(t, k), ints(need // 4) if need else None
 
 
 def _ptr(t: torch.Tensor | None):
@@ -94,7 +93,8 @@ def moe_route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax",
         logits = logits.contiguous()   # rows that share memory (an expanded matrix)
     weights = torch.empty((t, top_k), dtype=torch.float32, device=logits.device)
     experts = torch.empty((t, top_k), dtype=torch.int32, device=logits.device)
-    offsets, tokens, places, ws, need = _order_outputs(t, e, top_k, logits.device)
+    need = _lib.lib().i8l_moe_route_workspace_bytes(t, e, top_k)
+    offsets, tokens, places, ws = _order_outputs(t, e, top_k, need, logits.device)
     with torch.cuda.device(logits.device):
         status = _lib.lib().i8l_moe_route(
             logits.data_ptr(), _ld(logits), code, t, e, top_k, SCORING.index(scoring),
@@ -123,7 +123,8 @@ def moe_order(experts: torch.Tensor, n_experts: int):
     if n_experts < 1 or k < 1:
         raise ValueError(f"{k} choices of {n_experts} experts")
     experts = experts.contiguous()
-    offsets, tokens, places, ws, need = _order_outputs(t, n_experts, k, experts.device)
+    need = _lib.lib().i8l_moe_order_workspace_bytes(t, n_experts, k)
+    offsets, tokens, places, ws = _order_outputs(t, n_experts, k, need, experts.device)
     with torch.cuda.device(experts.device):
         status = _lib.lib().i8l_moe_order(experts.data_ptr(), t, n_experts, k, offsets.data_ptr(),
                                           tokens.data_ptr(), places.data_ptr(), _ptr(ws), need,

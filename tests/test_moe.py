@@ -54,8 +54,8 @@ def test_route_entry_refuses():
     assert call(dt=_lib.I32) == BAD and call(scoring=2) == BAD and call(scoring=-1) == BAD
     assert call(E=513, ldl=513) == BAD and call(E=100, ldl=100, k=65) == BAD
     assert call(T=2 ** 25, k=2) == BAD
-    need = L.i8l_moe_order_workspace_bytes(2000, 8, 2)
-    assert need > 0 and L.i8l_moe_order_workspace_bytes(1, 8, 2) == 0
+    need = L.i8l_moe_route_workspace_bytes(2000, 8, 2)
+    assert need > 0 and L.i8l_moe_route_workspace_bytes(1, 8, 2) == 0
     assert call(T=2000) == INV and call(T=2000, ws=P, nbytes=need - 1) == INV
     assert call(T=2000, ws=ctypes.c_void_p(0x1002), nbytes=need) == INV
 
@@ -70,7 +70,7 @@ def test_order_entry_refuses():
     assert call(E=513) == BAD and call(k=65) == BAD and call(T=2 ** 24 + 1) == BAD
     assert call(T=2000) == INV                                        # no workspace
     for sizes in ((-1, 8, 2), (2000, 0, 2), (2000, 8, 0), (2000, 513, 2), (2000, 8, 65)):
-        assert L.i8l_moe_order_workspace_bytes(*sizes) == 0
+        assert L.i8l_moe_order_workspace_bytes(*sizes) == 0 == L.i8l_moe_route_workspace_bytes(*sizes)
 
 
 def test_grouped_entry_refuses():
