@@ -127,7 +127,7 @@ bool grouped_fast_ok(const Grouped& p) {
   return p.K % 16 == 0 && aligned16(p.a) && aligned16(p.b) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
          p.eb % 16 == 0 && p.N % (p.silu ? 16 : 8) == 0 && aligned16(p.sb) && aligned16(p.bias) &&
          aligned16(p.out) && p.ldc * es % 16 == 0 && (int64_t)p.M * p.lda + 2 * p.K < most &&
-         (int64_t)p.N * p.ldb + 2 * p.K < most &&
+         (int64_t)p.N * p.ldb + 2 * p.K < most && p.ldc * es < ((int64_t)1 << 22) &&
          (most_blocks(p.R, p.E, 16) + 1) * ((p.N + 31) / 32) < (1 << 22);
 }
 

@@ -25,11 +25,15 @@ namespace {
 // vmcnt (all but the newest five halves have landed: the next phase's reads) and one workgroup
 // barrier, which makes both true of every wave.
 //
+// A half is BM / 2 rows in a row, so a tile of no more rows than that (an expert's last) leaves out the
+// MFMAs of phases 2 and 3.
+//
 // The workgroups walk the tiles of all experts; the copies of a tile's last two steps are the next
 // tile's first two, so they fly during the epilogue, which every wave does alone through its own 4 KiB
-// of LDS.  What a tile needs to be found stands in LDS: the experts' first blocks and rows, and the
-// source rows of three tiles (read an epilogue ahead, where nothing but stores is in flight, so that
-// no wait for them drains the copies).
+// of LDS.  What the epilogue reads stands in LDS before it begins (the tile's scales and bias, and the
+// experts' first blocks and rows, by which tiles are found), since a wait for a load would be one for
+// the copies requested before it; it is fetched an epilogue ahead, the rows' indices two, behind the
+// copies and awaited with them when half of the stores are out.
 //
 // Rows past the expert's last, whole steps past K and its tail within a step are read outside the
 // buffers, as zeros, at the price of one instruction a copy (zeros toggle nothing: they cost little of
@@ -40,7 +44,19 @@ struct PhasedShared {
   int32_t first[kMaxExperts + 1];            // an expert's first block; [E]: their number
   int32_t lo[kMaxExperts], hi[kMaxExperts];  // its rows
   int32_t source[3][256];                    // a tile's rows of A; -1: past the expert's last
+  GroupTile tile[3];                         // the tiles whose source rows those are
+  alignas(16) float sa[2][256], sb[2][256], bias[2][256];   // a tile's rows' and columns'
 };
+
+constexpr int kStoreCpol = 2;   // non-temporal: the next kernel's reads, if any, are far behind
+
+// The lane's number, counted where it is asked for: a value derived from it there is neither kept in
+// registers over the main loop nor, worse, out of them (a reload waits for the copies in flight).
+__device__ __forceinline__ int fresh_lane() {
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(l));
+  return l;
+}
 
 constexpr int kBadRow = -2;   // a source row outside [0, M): zeros, and NaN in the end
 
@@ -50,13 +66,14 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
   constexpr int QN = 2 * QB;                         // column fragments of a wave
   constexpr int BM = WM * 64 * QA, BN = WN * 32 * QN, BK = kStep;
   constexpr int BNO = SILU ? BN / 2 : BN;            // output columns
+  static_assert(BN == 256 && BM <= 256, "a thread a row and a column");
   constexpr int CPR = BK / 16, RPC = 64 / CPR;       // chunks of a row, rows of a copy
   constexpr int KK = BK / 32;                        // MFMA substeps of a step
   constexpr int HA = BM / 2 * BK, HB = BN / 2 * BK;  // bytes of a half
   constexpr int JA = HA / 1024 / W, JB = HB / 1024 / W;   // copies a wave
   constexpr int B0 = 4 * HA, SB = 2 * HB;            // LDS: A [buffer][half], then B, then staging
   constexpr int STG = B0 + 2 * SB;
-  static_assert(JA >= 1 && JB >= 1 && BM <= 256, "whole copies");
+  static_assert(JA >= 1 && JB >= 1, "whole copies");
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];
   PhasedShared& sh = *(PhasedShared*)(lds + STG + W * 4096);
 
@@ -85,15 +102,24 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
   __syncthreads();
   const int total_blocks = __builtin_amdgcn_readfirstlane(sh.first[p.E]);
   const int64_t total64 = (int64_t)total_blocks * cols;
-  const int tiles = (int)min(total64, (int64_t)INT32_MAX);
+  const int tiles = __builtin_amdgcn_readfirstlane((int)min(total64, (int64_t)INT32_MAX));
   if ((int)blockIdx.x >= tiles) return;
+  const int stride = gridDim.x;   // (a tile's number plus two of these stays below 2^31: see the launch)
 
   // Tile `t` of this walk: consecutive positions go to one XCD, and within an expert up to 8 row blocks
-  // are walked together, so that what runs at a time shares weight and activation rows in L2.
+  // are walked together, so that what runs at a time shares weight and activation rows in L2.  Each
+  // round of an XCD's workgroups is turned by one against the last, so that none of them meets only
+  // full tiles and none only last ones.
+  const int group = stride / 8;
+  auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };   // (it is: said to the compiler)
   auto tile_at = [&](int t) {
+    const int round = group ? t / 8 / group : 0;
+    if (group && stride % 8 == 0 && (round + 1) * group * 8 <= tiles)
+      t = (round * group + (t / 8 + round) % group) * 8 + t % 8;
     const int pos = xcd_order(t, tiles);
     const int q = pos / cols;
     const int per = (p.E + 63) / 64;
+    const int lane = fresh_lane();
     const uint64_t m1 = __ballot(sh.first[min((lane + 1) * per, p.E)] > q);
     const int g = __builtin_ctzll(m1) * per;
     const uint64_t m2 = __ballot(sh.first[min(g + lane + 1, p.E)] > q);
@@ -107,49 +133,42 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
     constexpr int GM = 8;
     const int first = local / (GM * cols) * GM, gsize = min(nb - first, GM);
     const int in = local - first * cols;
-    o.col = in / gsize;
-    o.row0 = lo + (first + in % gsize) * BM;
-    o.end = min(o.row0 + BM, hi);
+    o.col = uniform(in / gsize);
+    o.row0 = uniform(lo + (first + in % gsize) * BM);
+    o.end = uniform(min(o.row0 + BM, hi));
     return o;
   };
-  // a tile's source rows: row tid of it
-  auto source_of = [&](const GroupTile& g) {
-    if (tid >= BM) return -1;
-    const int i = g.row0 + tid;
+  // a tile's source rows: row x of it
+  auto source_of = [&](const GroupTile& g, int x) {
+    if (x >= BM) return -1;
+    const int i = g.row0 + x;
     if (i >= g.end) return -1;
     const int r = p.rows ? p.rows[i] : i;
     return r >= 0 && r < p.M ? r : kBadRow;
   };
 
   // Copies: copy j of a half writes LDS rows [RPC x, RPC x + RPC), x = W j + wave; lane l writes
-  // slot l % CPR of row l / CPR.  Half row r lies in wave block r / R of that half (R rows each).
-  const int lrow = lane / CPR;
-  const int chunk = ((lane % CPR) ^ swz<BK>(wave * RPC + lrow)) * 16;
+  // slot l % CPR of row l / CPR.  B's half row r lies in wave block r / R of that half (R rows each).
   static_assert((W * RPC) % 16 == 0, "the swizzle must not depend on j");
   const int lda32 = (int)p.lda, ldb32 = (int)p.ldb;
-  int arow[2][JA], brow[2][JB];   // tile rows; the weight's byte offsets in the tile being requested
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int j = 0; j < JA; ++j) {
-      constexpr int RA = 32 * QA;
-      const int r = (W * j + wave) * RPC;
-      arow[h][j] = (r / RA) * (2 * RA) + h * RA + r % RA;
-    }
+  int brow[2][JB];         // the weight's byte offsets in the tile being requested
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_i8*)lds + wave * 1024;
-  const uint32_t voffB = (uint32_t)(lrow * ldb32 + chunk);
+  int lrow, chunk;
+  uint32_t voffB;
   const v4u bufA = buffer_of(p.a, abytes);
   v4u bufB = bufA;
   uint32_t voffA[2][JA];
-  int kreq = 0;            // the K position being requested
+  int kreq;                // the K position being requested
   uint32_t past = 0;       // kOutside in the lanes whose chunk of that step lies past K
-  auto request_from = [&](const GroupTile& g, int buf) {
+  // (found again at the start of the tile, rather than kept over the epilogue)
+  auto request_from = [&](const GroupTile& g, int buf, int k) {
+    kreq = k;
     bufB = buffer_of(p.b + g.e * p.eb, bbytes);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int j = 0; j < JA; ++j) {
-        const int r = sh.source[buf][arow[h][j] + lrow];
+        const int r = sh.source[buf][h * (BM / 2) + (W * j + wave) * RPC + lrow];
         voffA[h][j] = r >= 0 ? (uint32_t)(r * lda32 + chunk) : kOutside;
       }
       constexpr int RB = 32 * QB;
@@ -159,10 +178,9 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
         const int r = (W * j + wave) * RPC, x = r / RB, y = r % RB;
         const int n = SILU ? h * width + min(g.col * BNO + x * RB + y, width - 8)
                            : min(g.col * BN + x * (2 * RB) + h * RB + y, width - 8);
-        brow[h][j] = n * ldb32;
+        brow[h][j] = uniform(n * ldb32);
       }
     }
-    kreq = 0;
   };
   auto begin_step = [&] { past = kreq + chunk < p.K ? 0u : kOutside; };
   // copy j of A's / B's half h of the step being requested, into buffer buf
@@ -174,10 +192,17 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
   };
 
   // Fragment reads: lane l reads row l%32 of a 32-row block, chunk 2*kk + l/32.
-  const int frow = lane & 31, fhalf = lane >> 5;
   int ofs[KK];
+  // what the main loop derives from the lane, anew for each tile
+  auto lay_out = [&] {
+    const int l = fresh_lane();
+    lrow = l / CPR;
+    chunk = ((l % CPR) ^ swz<BK>(wave * RPC + lrow)) * 16;
+    voffB = (uint32_t)(lrow * ldb32 + chunk);
+    const int frow = l & 31, fhalf = l >> 5;
 #pragma unroll
-  for (int kk = 0; kk < KK; ++kk) ofs[kk] = frow * BK + (((2 * kk + fhalf) ^ swz<BK>(frow)) * 16);
+    for (int kk = 0; kk < KK; ++kk) ofs[kk] = frow * BK + (((2 * kk + fhalf) ^ swz<BK>(frow)) * 16);
+  };
   const int8_t* la = lds + wm * 32 * QA * BK;
   const int8_t* lb = lds + B0 + wn * 32 * QB * BK;
   v4i fa[2][QA][KK], fb[2][QB][KK];
@@ -192,12 +217,19 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
       fb[h][i][kk] = *(const v4i*)(lb + ofs[kk] + buf * SB + h * HB + i * 32 * BK);
   };
 
-  v16i acc[2][2][QA][QB];
   // A phase's work: per MFMA substep its MFMAs with the next phase's reads of that substep between
   // them, and one in KK of its copies.  zero: a tile's first step, whose first substep starts from 0.
-  auto body = [&](auto hac, auto hbc, auto zero, auto read, int reads, auto copy, auto copies) {
+  typedef v16i Sums[2][2][QA][QB];
+  auto body = [&](Sums& acc, auto hac, auto hbc, auto fullc, auto zero, auto read, int reads, auto copy, auto copies) {
     constexpr int ha = decltype(hac)::value, hb = decltype(hbc)::value;
     constexpr int NC = decltype(copies)::value;
+    if constexpr (ha == 1 && !decltype(fullc)::value) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) read(kk);
+#pragma unroll
+      for (int j = 0; j < NC; ++j) copy(j);
+      return;
+    }
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
 #pragma unroll
@@ -220,12 +252,12 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
   };
   // One K step of parity `par`.  TAIL: a tile's last (it reads nothing ahead).  HEAD: 4 for a
   // tile's first step and 1 for its second, the phases that `landed` spares the wait for copies
-  // (a workgroup's later tiles find them landed).
+  // (a workgroup's later tiles find them landed).  fullc: the tile has rows in A's half 1.
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
   typedef std::integral_constant<int, JA> NJA;
   typedef std::integral_constant<int, JB> NJB;
-  auto step = [&](auto par, auto tail, auto headc, bool landed) {
+  auto step = [&](Sums& acc, auto par, auto tail, auto headc, auto fullc, bool landed) {
     constexpr int f = decltype(par)::value, s = 1 - f;
     constexpr bool TAIL = decltype(tail)::value;
     constexpr int HEAD = decltype(headc)::value;
@@ -244,14 +276,14 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
       lds_barrier();
     };
     begin_step();
-    body(I0{}, HF{}, zero, [&](int kk) { readB(s, f, kk); }, QB, [&](int j) { copyA(0, f, j); }, NJA{});
+    body(acc, I0{}, HF{}, fullc, zero, [&](int kk) { readB(s, f, kk); }, QB, [&](int j) { copyA(0, f, j); }, NJA{});
     phase_end(I0{}, std::integral_constant<int, NA>{});
-    body(I0{}, HS{}, zero, [&](int kk) { readA(1, f, kk); }, QA, [&](int j) { copyB(f, f, j); }, NJB{});
+    body(acc, I0{}, HS{}, fullc, zero, [&](int kk) { readA(1, f, kk); }, QA, [&](int j) { copyB(f, f, j); }, NJB{});
     phase_end(I1{}, std::integral_constant<int, NB>{});
-    body(I1{}, HS{}, zero, [&](int kk) { if constexpr (!TAIL) readA(0, 1 - f, kk); }, TAIL ? 0 : QA,
+    body(acc, I1{}, HS{}, fullc, zero, [&](int kk) { if constexpr (!TAIL) readA(0, 1 - f, kk); }, TAIL ? 0 : QA,
          [&](int j) { copyB(s, f, j); }, NJB{});
     if constexpr (!TAIL) phase_end(std::integral_constant<int, 2>{}, std::integral_constant<int, NB>{});
-    body(I1{}, HF{}, zero, [&](int kk) { if constexpr (!TAIL) readB(s, 1 - f, kk); }, TAIL ? 0 : QB,
+    body(acc, I1{}, HF{}, fullc, zero, [&](int kk) { if constexpr (!TAIL) readB(s, 1 - f, kk); }, TAIL ? 0 : QB,
          [&](int j) { copyA(1, f, j); }, NJA{});
     if constexpr (!TAIL) phase_end(std::integral_constant<int, 3>{}, std::integral_constant<int, NA>{});
     kreq += BK;
@@ -266,20 +298,59 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
     kreq += BK;
   };
 
-  int tile = blockIdx.x, buf = 0;   // buf: where the tile's source rows stand
-  GroupTile g0 = tile_at(tile), g1 = g0;
-  bool more = tile + (int)gridDim.x < tiles;   // (tile + gridDim.x stays below 2^31: see the launch)
-  if (more) g1 = tile_at(tile + gridDim.x);
-  if (tid < BM) {
-    sh.source[0][tid] = source_of(g0);
-    sh.source[1][tid] = source_of(g1);
+  // the tile in a slot of the tables
+  auto tile_in = [&](int slot) {
+    const GroupTile& t = sh.tile[slot];
+    return GroupTile{uniform(t.e), uniform(t.row0), uniform(t.end), uniform(t.col)};
+  };
+  // a tile's scales and bias: row x's, column x's
+  struct Operands {
+    float sa, sb;
+    uint32_t bias;
+  };
+  auto operands_of = [&](const GroupTile& g, int source, int x) {
+    Operands o;
+    o.sa = p.sa[p.sa_per_row ? max(source, 0) : 0];
+    int n = g.col * BNO + x % BNO;
+    n = min(n, width - 1) + (SILU && x >= BNO ? width : 0);
+    const int64_t at = (int64_t)g.e * p.N + n;
+    o.sb = p.sb[at];
+    o.bias = 0;
+    if constexpr (BIAS)
+      o.bias = p.bias_dtype == I8L_F32 ? ((const uint32_t*)p.bias)[at] : ((const uint16_t*)p.bias)[at];
+    return o;
+  };
+  auto keep = [&](int half, int source, const Operands& o, int x) {
+    if (x < BM) sh.sa[half][x] = source == kBadRow ? __builtin_nanf("") : o.sa;
+    sh.sb[half][x] = o.sb;
+    if constexpr (BIAS)
+      sh.bias[half][x] =
+          p.bias_dtype == I8L_F32 ? __uint_as_float(o.bias) : act_to_f32(o.bias, p.bias_dtype);
+  };
+  {
+    const GroupTile g0 = tile_at(blockIdx.x);
+    const GroupTile g1 = (int)blockIdx.x + stride < tiles ? tile_at(blockIdx.x + stride) : g0;
+    const int s0 = source_of(g0, tid), s1 = source_of(g1, tid);
+    keep(0, s0, operands_of(g0, s0, tid), tid);
+    if (tid < BM) {
+      sh.source[0][tid] = s0;
+      sh.source[1][tid] = s1;
+    }
+    if (tid == 0) sh.tile[0] = g0, sh.tile[1] = g1;
+    __syncthreads();
+    lay_out();
+    request_from(g0, 0, 0);
+    request_step(I0{});
+    request_step(I1{});
   }
-  __syncthreads();
-  request_from(g0, 0);
-  request_step(I0{});
-  request_step(I1{});
-  bool landed = false;
-  for (;;) {
+  // Tile number `tile`, the workgroup's nth, up to the start of the next.  fullc: it has rows in A's
+  // half 1.  Slots n % 3 and n % 2 of the tables are its own.
+  auto run_tile = [&](auto fullc, const GroupTile& g0, int tile, int n) {
+    const int rows = g0.end - g0.row0, half = n & 1;
+    const int buf = n % 3, buf1 = (n + 1) % 3, buf2 = (n + 2) % 3;
+    const bool landed = n > 0;
+    lay_out();
+    request_from(g0, buf, 2 * BK);
     // A0(0) and B0(0) into registers, then the steps in pairs, the first and the last apart
     if (!landed) wait_vmcnt<3 * JA + 3 * JB>();
     lds_barrier();
@@ -294,113 +365,141 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
 
     // the copies awaited in the first five phases were requested before the previous tile's
     // stores, whose epilogue waited for them
-    step(I0{}, std::false_type{}, std::integral_constant<int, 4>{}, landed);
-    step(I1{}, std::false_type{}, I1{}, landed);
+    Sums acc;
+    step(acc, I0{}, std::false_type{}, std::integral_constant<int, 4>{}, fullc, landed);
+    step(acc, I1{}, std::false_type{}, I1{}, fullc, landed);
     for (int t = 2; t + 2 < KT; t += 2) {
-      step(I0{}, std::false_type{}, I0{}, false);
-      step(I1{}, std::false_type{}, I0{}, false);
+      step(acc, I0{}, std::false_type{}, I0{}, fullc, false);
+      step(acc, I1{}, std::false_type{}, I0{}, fullc, false);
     }
-    const int buf1 = buf == 2 ? 0 : buf + 1, buf2 = buf1 == 2 ? 0 : buf1 + 1;
-    request_from(g1, buf1);   // (past the last tile: one of its rows again, not used)
-    step(I0{}, std::false_type{}, I0{}, false);
-    step(I1{}, std::true_type{}, I0{}, false);
+    request_from(tile_in(buf1), buf1, 0);   // (past the last tile: an earlier one again, not used)
+    step(acc, I0{}, std::false_type{}, I0{}, fullc, false);
+    step(acc, I1{}, std::true_type{}, I0{}, fullc, false);
 
     // ---- epilogue: acc * scale_a * scale_b (+ bias) in fp32, left to right, then one cast.
     // Each wave takes 32 rows x 64 columns (16-bit outputs; 32 columns of 4-byte ones) at a time
     // through its 4 KiB: rows of 128 bytes, chunk c at slot c ^ (row & 7), written out in whole
-    // 128-byte lines, 8 rows a store.  The lane index is taken anew, opaque, so that what the
-    // epilogue derives from it is not kept in registers over the main loop.
-    int ln = lane;
-    asm volatile("" : "+v"(ln));
+    // 128-byte lines, 8 rows a store, while the next 32 rows are computed.  The stores are buffer
+    // stores, which drop what lies outside the problem and are issued whatever the mask: the wait
+    // behind the first of them counts them.
+    const int ln = fresh_lane();
     const int erow = ln & 31, ehalf = ln >> 5, srow = ln >> 3, sch = ln & 7;
     constexpr int FN = SILU ? QB : QN;                // output fragments across
-    const int nw = g0.col * BNO + wn * 32 * FN, mw = wm * 64 * QA;
-    int8_t* stg = lds + STG + wave * 4096;
-    const int64_t ecol = (int64_t)g0.e * p.N;
-    float sam[2][QA];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < QA; ++i) {
-        const int r = sh.source[buf][mw + (h * QA + i) * 32 + erow];
-        const float s = p.sa[p.sa_per_row ? max(r, 0) : 0];
-        sam[h][i] = r == kBadRow ? __builtin_nanf("") : s;
-      }
-    // every copy in flight (the next tile's first two steps) has landed past here, so the next
-    // tile's first waits need not count past this tile's stores
-    wait_vmcnt<0>();
-    asm volatile("" ::: "memory");
-    // the tile after the next one, and its source rows
-    const bool more2 = more && tile + 2 * (int64_t)gridDim.x < tiles;
-    GroupTile g2 = g1;
-    if (more2) g2 = tile_at(tile + 2 * gridDim.x);
-    const int src2 = source_of(g2);
+    constexpr int ES = OD == I8L_F32 ? 4 : 2, EPC = 16 / ES;   // bytes of an element, elements of a chunk
     constexpr int FG = OD == I8L_F32 ? 1 : 2;         // fragments at a time
+    constexpr int PER = FN < FG ? FN : FG;
+    const int cw = wn * 32 * FN, nw = g0.col * BNO + cw;
+    int8_t* stg = lds + STG + wave * 4096;
+    const auto bufC = __builtin_amdgcn_make_buffer_rsrc((char*)p.out + (int64_t)g0.row0 * p.ldc * ES, 0,
+                                                        0x7fffffff, 0x00020000);
+    // the tile after the next one and its source rows, and the next one's scales
+    const GroupTile g1 = tile_in(buf1);
+    const GroupTile g2 = tile + 2 * stride < tiles ? tile_at(tile + 2 * stride) : g1;
+    const int td = 64 * wave + ln;
+    const int src1 = td < BM ? sh.source[buf1][td] : -1;
+    const int src2 = source_of(g2, td);
+    const Operands next = operands_of(g1, src1, td);
+    constexpr int NB = decltype(fullc)::value ? 2 * QA : QA;   // blocks of 32 rows
+    // (every load is requested before the first store, so the wait behind the stores covers them)
+    asm volatile("" ::: "memory");
 #pragma unroll
-    for (int x0 = 0; x0 < FN; x0 += FG) {
-      constexpr int PER = FN < FG ? FN : FG;
-      ColQuad cl[PER][4], cu[SILU ? PER : 1][4];
+    for (int x0 = 0; x0 < FN; x0 += PER) {
+      v4i pack[2][PER][OD == I8L_F32 ? 4 : 2];        // a block's values as stored, one ahead
+      auto compute = [&](int b, v4i (&o)[PER][OD == I8L_F32 ? 4 : 2]) {
+        const int h = b / QA, i = b % QA;
+        const float sam = sh.sa[half][h * (BM / 2) + (wm * QA + i) * 32 + erow];
 #pragma unroll
-      for (int c = 0; c < PER; ++c)
+        for (int c = 0; c < PER; ++c)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = nw + 32 * (x0 + c) + 8 * q + 4 * ehalf;
-          cl[c][q] = load_quad<BIAS>(p, ecol, SILU ? min(n, width - 4) : n);
-          if constexpr (SILU) cu[c][q] = load_quad<BIAS>(p, ecol, width + min(n, width - 4));
-        }
+          for (int q = 0; q < 4; ++q) {
+            const int x = x0 + c, col = cw + 32 * x + 8 * q + 4 * ehalf;
+            const float4 s0 = *(const float4*)&sh.sb[half][col];
+            const float4 s1 = *(const float4*)&sh.sb[half][SILU ? BNO + col : col];
+            float4 b0 = {}, b1 = {};
+            if constexpr (BIAS) {
+              b0 = *(const float4*)&sh.bias[half][col];
+              b1 = *(const float4*)&sh.bias[half][SILU ? BNO + col : col];
+            }
+            float v[4];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < QA; ++i) {
-          const int mb = g0.row0 + mw + (h * QA + i) * 32;
-#pragma unroll
-          for (int c = 0; c < PER; ++c) {
-            const int x = x0 + c;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float v[4];
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                if constexpr (SILU) {
-                  v[r] = silu_mul<OD == I8L_F32>(
-                      quad_value<BIAS>(acc[h][0][i][x][4 * q + r], sam[h][i], cl[c][q], r),
-                      quad_value<BIAS>(acc[h][1][i][x][4 * q + r], sam[h][i], cu[c][q], r));
-                } else {
-                  v[r] = quad_value<BIAS>(acc[h][x / QB][i][x % QB][4 * q + r], sam[h][i], cl[c][q], r);
-                }
-                // the value itself is rounded to fp16 in a cast of its own: opaque, or the product
-                // and the cast become one v_fma_mixlo_f16, which rounds once
-                if constexpr (OD == I8L_F16) asm volatile("" : "+v"(v[r]));
-              }
-              if constexpr (OD == I8L_F32)
-                *(float4*)(stg + erow * 128 + (((2 * q + ehalf) ^ (erow & 7)) * 16)) =
-                    make_float4(v[0], v[1], v[2], v[3]);
+            for (int r = 0; r < 4; ++r) {
+              auto scaled = [&](int32_t a, const float4& s, const float4& b) {
+                float y = (float)a;
+                y = y * sam;
+                y = y * (r == 0 ? s.x : r == 1 ? s.y : r == 2 ? s.z : s.w);
+                if constexpr (BIAS) y = y + (r == 0 ? b.x : r == 1 ? b.y : r == 2 ? b.z : b.w);
+                return y;
+              };
+              if constexpr (SILU)
+                v[r] = silu_mul<OD == I8L_F32>(scaled(acc[h][0][i][x][4 * q + r], s0, b0),
+                                               scaled(acc[h][1][i][x][4 * q + r], s1, b1));
               else
-                *(uint2*)(stg + erow * 128 + (((4 * c + q) ^ (erow & 7)) * 16) + 8 * ehalf) =
-                    make_uint2(f32x2_to_act2<OD>(v[0], v[1]), f32x2_to_act2<OD>(v[2], v[3]));
+                v[r] = scaled(acc[h][x / QB][i][x % QB][4 * q + r], s0, b0);
+              // the value itself is rounded to fp16 in a cast of its own: opaque, or the product
+              // and the cast become one v_fma_mixlo_f16, which rounds once
+              if constexpr (OD == I8L_F16) asm volatile("" : "+v"(v[r]));
+            }
+            if constexpr (OD == I8L_F32) {
+              o[c][q] = __builtin_bit_cast(v4i, make_float4(v[0], v[1], v[2], v[3]));
+            } else {
+              o[c][q / 2][q % 2 * 2] = (int)f32x2_to_act2<OD>(v[0], v[1]);
+              o[c][q / 2][q % 2 * 2 + 1] = (int)f32x2_to_act2<OD>(v[2], v[3]);
             }
           }
-          constexpr int EPC = OD == I8L_F32 ? 4 : 8;   // elements of a chunk
-          const int n = nw + 32 * x0 + EPC * sch;
+      };
+      auto stage = [&](const v4i (&o)[PER][OD == I8L_F32 ? 4 : 2]) {
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int row = 8 * y + srow;
-            const v4i v = *(const v4i*)(stg + row * 128 + ((sch ^ srow) * 16));
-            if (mb + row < g0.end && n < width && sch * EPC < 32 * PER)
-              __builtin_nontemporal_store(
-                  v, (v4i*)((char*)p.out + ((mb + row) * p.ldc + n) * (OD == I8L_F32 ? 4 : 2)));
+        for (int c = 0; c < PER; ++c)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if constexpr (OD == I8L_F32)
+              *(v4i*)(stg + erow * 128 + (((2 * q + ehalf) ^ (erow & 7)) * 16)) = o[c][q];
+            else
+              *(uint2*)(stg + erow * 128 + (((4 * c + q) ^ (erow & 7)) * 16) + 8 * ehalf) =
+                  make_uint2((uint32_t)o[c][q / 2][q % 2 * 2], (uint32_t)o[c][q / 2][q % 2 * 2 + 1]);
           }
+      };
+      auto store = [&](int b) {
+        const int row0 = b / QA * (BM / 2) + (wm * QA + b % QA) * 32;
+        const int n = nw + 32 * x0 + EPC * sch;
+        const bool in = n < width && sch * EPC < 32 * PER;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int row = 8 * y + srow;
+          const v4i v = *(const v4i*)(stg + row * 128 + ((sch ^ srow) * 16));
+          const uint32_t at = (uint32_t)(((row0 + row) * (int)p.ldc + n) * ES);
+          __builtin_amdgcn_raw_buffer_store_b128(
+              __builtin_bit_cast(v4u, v), bufC,
+              in && row0 + row < rows ? at : kOutside, 0, kStoreCpol);
         }
-      asm volatile("" ::: "memory");   // the next columns' operands load after these
+      };
+      compute(0, pack[0]);
+      stage(pack[0]);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        if (b + 1 < NB) compute(b + 1, pack[(b + 1) % 2]);
+        __builtin_amdgcn_sched_barrier(0);            // (else the registers of several blocks live at a time)
+        store(b);
+        if (b + 1 < NB) stage(pack[(b + 1) % 2]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (x0 == 0) {
+        // the loads above and every copy in flight (the next tile's first two steps) have landed past
+        // here, so the next tile's first waits need not count past this tile's stores
+        asm volatile("" ::: "memory");
+        wait_vmcnt<4 * NB>();
+        asm volatile("" ::: "memory");
+      }
     }
-    if (!more) break;
-    if (tid < BM) sh.source[buf2][tid] = src2;
-    tile += gridDim.x;
-    buf = buf1;
-    more = more2;
-    g0 = g1;
-    g1 = g2;
-    landed = true;
+    keep(half ^ 1, src1, next, td);
+    if (td < BM) sh.source[buf2][td] = src2;
+    if (td == 0) sh.tile[buf2] = g2;
+  };
+  // (the sums of the two kinds of tile never meet, so that each keeps its registers)
+  for (int n = 0, tile = blockIdx.x; tile < tiles; ++n, tile += stride) {
+    const GroupTile g = tile_in(n % 3);
+    if (g.end - g.row0 > BM / 2) run_tile(std::true_type{}, g, tile, n);
+    else run_tile(std::false_type{}, g, tile, n);
   }
 }
 
