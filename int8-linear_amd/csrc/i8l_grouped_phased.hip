@@ -40,11 +40,13 @@ namespace {
 // the power that bounds the multiplications).
 constexpr int kStep = 128;
 
+constexpr int kTiles = 32;   // found half of them at a time, a tile a lane
+
 struct PhasedShared {
   int32_t first[kMaxExperts + 1];            // an expert's first block; [E]: their number
   int32_t lo[kMaxExperts], hi[kMaxExperts];  // its rows
   int32_t source[3][256];                    // a tile's rows of A; -1: past the expert's last
-  GroupTile tile[3];                         // the tiles whose source rows those are
+  GroupTile tile[kTiles];                    // the workgroup's tiles, its nth in slot n % kTiles
   alignas(16) float sa[2][256], sb[2][256], bias[2][256];   // a tile's rows' and columns'
 };
 
@@ -56,6 +58,12 @@ __device__ __forceinline__ int fresh_lane() {
   int l;
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(l));
   return l;
+}
+
+// p[i] by a scalar base and a 32-bit byte offset.
+template <typename T>
+__device__ __forceinline__ T at32(const T* p, int i) {
+  return *(const T*)((const char*)p + (uint32_t)i * (uint32_t)sizeof(T));
 }
 
 constexpr int kBadRow = -2;   // a source row outside [0, M): zeros, and NaN in the end
@@ -104,46 +112,48 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
   const int64_t total64 = (int64_t)total_blocks * cols;
   const int tiles = __builtin_amdgcn_readfirstlane((int)min(total64, (int64_t)INT32_MAX));
   if ((int)blockIdx.x >= tiles) return;
-  const int stride = gridDim.x;   // (a tile's number plus two of these stays below 2^31: see the launch)
+  const int stride = gridDim.x;
 
-  // Tile `t` of this walk: consecutive positions go to one XCD, and within an expert up to 8 row blocks
+  // Tile t of all: consecutive positions go to one XCD, and within an expert up to 8 row blocks
   // are walked together, so that what runs at a time shares weight and activation rows in L2.  Each
   // round of an XCD's workgroups is turned by one against the last, so that none of them meets only
   // full tiles and none only last ones.
-  const int group = stride / 8;
   auto uniform = [](int v) { return __builtin_amdgcn_readfirstlane(v); };   // (it is: said to the compiler)
-  auto tile_at = [&](int t) {
+  const int group = stride / 8;
+  auto tile_at = [&](int t) {   // t: a lane's own
     const int round = group ? t / 8 / group : 0;
     if (group && stride % 8 == 0 && (round + 1) * group * 8 <= tiles)
       t = (round * group + (t / 8 + round) % group) * 8 + t % 8;
     const int pos = xcd_order(t, tiles);
     const int q = pos / cols;
-    const int per = (p.E + 63) / 64;
-    const int lane = fresh_lane();
-    const uint64_t m1 = __ballot(sh.first[min((lane + 1) * per, p.E)] > q);
-    const int g = __builtin_ctzll(m1) * per;
-    const uint64_t m2 = __ballot(sh.first[min(g + lane + 1, p.E)] > q);
     GroupTile o;
-    o.e = __builtin_amdgcn_readfirstlane(g + __builtin_ctzll(m2));
-    const int f = __builtin_amdgcn_readfirstlane(sh.first[o.e]);
-    const int nb = __builtin_amdgcn_readfirstlane(sh.first[o.e + 1]) - f;
-    const int lo = __builtin_amdgcn_readfirstlane(sh.lo[o.e]);
-    const int hi = __builtin_amdgcn_readfirstlane(sh.hi[o.e]);
+    o.e = 0;                    // the last expert whose first block is not behind q
+#pragma unroll
+    for (int step = kMaxExperts / 2; step; step /= 2)
+      if (o.e + step < p.E && sh.first[o.e + step] <= q) o.e += step;
+    const int f = sh.first[o.e], nb = sh.first[o.e + 1] - f;
     const int local = pos - f * cols;
     constexpr int GM = 8;
     const int first = local / (GM * cols) * GM, gsize = min(nb - first, GM);
     const int in = local - first * cols;
-    o.col = uniform(in / gsize);
-    o.row0 = uniform(lo + (first + in % gsize) * BM);
-    o.end = uniform(min(o.row0 + BM, hi));
+    o.col = in / gsize;
+    o.row0 = sh.lo[o.e] + (first + in % gsize) * BM;
+    o.end = min(o.row0 + BM, sh.hi[o.e]);
     return o;
+  };
+  // The workgroup's tiles n .. n + count - 1 into the table, by one wave; past the last: the last again.
+  auto find_tiles = [&](int n, int count, int l) {
+    if (l < count) {
+      const int last = (tiles - 1 - (int)blockIdx.x) / stride;
+      sh.tile[(n + l) % kTiles] = tile_at(blockIdx.x + min(n + l, last) * stride);
+    }
   };
   // a tile's source rows: row x of it
   auto source_of = [&](const GroupTile& g, int x) {
     if (x >= BM) return -1;
     const int i = g.row0 + x;
     if (i >= g.end) return -1;
-    const int r = p.rows ? p.rows[i] : i;
+    const int r = p.rows ? at32(p.rows, i) : i;
     return r >= 0 && r < p.M ? r : kBadRow;
   };
 
@@ -298,9 +308,8 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
     kreq += BK;
   };
 
-  // the tile in a slot of the tables
-  auto tile_in = [&](int slot) {
-    const GroupTile& t = sh.tile[slot];
+  auto nth_tile = [&](int n) {
+    const GroupTile& t = sh.tile[n % kTiles];
     return GroupTile{uniform(t.e), uniform(t.row0), uniform(t.end), uniform(t.col)};
   };
   // a tile's scales and bias: row x's, column x's
@@ -310,14 +319,15 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
   };
   auto operands_of = [&](const GroupTile& g, int source, int x) {
     Operands o;
-    o.sa = p.sa[p.sa_per_row ? max(source, 0) : 0];
+    o.sa = at32(p.sa, p.sa_per_row ? max(source, 0) : 0);
     int n = g.col * BNO + x % BNO;
     n = min(n, width - 1) + (SILU && x >= BNO ? width : 0);
-    const int64_t at = (int64_t)g.e * p.N + n;
-    o.sb = p.sb[at];
+    const int64_t at = (int64_t)g.e * p.N;
+    o.sb = at32(p.sb + at, n);
     o.bias = 0;
     if constexpr (BIAS)
-      o.bias = p.bias_dtype == I8L_F32 ? ((const uint32_t*)p.bias)[at] : ((const uint16_t*)p.bias)[at];
+      o.bias = p.bias_dtype == I8L_F32 ? at32((const uint32_t*)p.bias + at, n)
+                                       : (uint32_t)at32((const uint16_t*)p.bias + at, n);
     return o;
   };
   auto keep = [&](int half, int source, const Operands& o, int x) {
@@ -327,25 +337,25 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
       sh.bias[half][x] =
           p.bias_dtype == I8L_F32 ? __uint_as_float(o.bias) : act_to_f32(o.bias, p.bias_dtype);
   };
+  if (wave == 0) find_tiles(0, kTiles, lane);
+  __syncthreads();
   {
-    const GroupTile g0 = tile_at(blockIdx.x);
-    const GroupTile g1 = (int)blockIdx.x + stride < tiles ? tile_at(blockIdx.x + stride) : g0;
+    const GroupTile g0 = nth_tile(0), g1 = nth_tile(1);
     const int s0 = source_of(g0, tid), s1 = source_of(g1, tid);
     keep(0, s0, operands_of(g0, s0, tid), tid);
     if (tid < BM) {
       sh.source[0][tid] = s0;
       sh.source[1][tid] = s1;
     }
-    if (tid == 0) sh.tile[0] = g0, sh.tile[1] = g1;
     __syncthreads();
     lay_out();
     request_from(g0, 0, 0);
     request_step(I0{});
     request_step(I1{});
   }
-  // Tile number `tile`, the workgroup's nth, up to the start of the next.  fullc: it has rows in A's
-  // half 1.  Slots n % 3 and n % 2 of the tables are its own.
-  auto run_tile = [&](auto fullc, const GroupTile& g0, int tile, int n) {
+  // The workgroup's nth tile, up to the start of the next.  fullc: it has rows in A's half 1.  Slots
+  // n % 3 and n % 2 of the rows' and operands' tables are its own.
+  auto run_tile = [&](auto fullc, const GroupTile& g0, int n) {
     const int rows = g0.end - g0.row0, half = n & 1;
     const int buf = n % 3, buf1 = (n + 1) % 3, buf2 = (n + 2) % 3;
     const bool landed = n > 0;
@@ -372,7 +382,7 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
       step(acc, I0{}, std::false_type{}, I0{}, fullc, false);
       step(acc, I1{}, std::false_type{}, I0{}, fullc, false);
     }
-    request_from(tile_in(buf1), buf1, 0);   // (past the last tile: an earlier one again, not used)
+    request_from(nth_tile(n + 1), buf1, 0);   // (past the last tile: an earlier one again, not used)
     step(acc, I0{}, std::false_type{}, I0{}, fullc, false);
     step(acc, I1{}, std::true_type{}, I0{}, fullc, false);
 
@@ -392,9 +402,8 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
     int8_t* stg = lds + STG + wave * 4096;
     const auto bufC = __builtin_amdgcn_make_buffer_rsrc((char*)p.out + (int64_t)g0.row0 * p.ldc * ES, 0,
                                                         0x7fffffff, 0x00020000);
-    // the tile after the next one and its source rows, and the next one's scales
-    const GroupTile g1 = tile_in(buf1);
-    const GroupTile g2 = tile + 2 * stride < tiles ? tile_at(tile + 2 * stride) : g1;
+    // the next tile's scales, and the source rows of the one after it
+    const GroupTile g1 = nth_tile(n + 1), g2 = nth_tile(n + 2);
     const int td = 64 * wave + ln;
     const int src1 = td < BM ? sh.source[buf1][td] : -1;
     const int src2 = source_of(g2, td);
@@ -493,13 +502,13 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
     }
     keep(half ^ 1, src1, next, td);
     if (td < BM) sh.source[buf2][td] = src2;
-    if (td == 0) sh.tile[buf2] = g2;
+    if (wave == 0 && (n + 1) % (kTiles / 2) == 0) find_tiles(n + 1 + kTiles / 2, kTiles / 2, ln);
   };
   // (the sums of the two kinds of tile never meet, so that each keeps its registers)
   for (int n = 0, tile = blockIdx.x; tile < tiles; ++n, tile += stride) {
-    const GroupTile g = tile_in(n % 3);
-    if (g.end - g.row0 > BM / 2) run_tile(std::true_type{}, g, tile, n);
-    else run_tile(std::false_type{}, g, tile, n);
+    const GroupTile g = nth_tile(n);
+    if (g.end - g.row0 > BM / 2) run_tile(std::true_type{}, g, n);
+    else run_tile(std::false_type{}, g, n);
   }
 }
 
