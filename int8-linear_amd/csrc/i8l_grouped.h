@@ -213,7 +213,8 @@ hipError_t launch_grouped_any(const Grouped& p, hipStream_t st);
 bool grouped_fast_ok(const Grouped& p);
 // Few rows an expert: 16, 32 or 64 rows x 64 columns (i8l_grouped_ring.hip).
 hipError_t launch_grouped_ring(int bm, const Grouped& p, hipStream_t st);
-// Macro tiles of bm = 64, 128 or 256 rows x 256 columns (i8l_grouped_phased.hip).
-hipError_t launch_grouped_phased(int bm, const Grouped& p, hipStream_t st);
+// Macro tiles of bm = 64, 128 or 256 rows x 256 columns (i8l_grouped_phased.hip).  stream (bm up to
+// 128): the weights past the caches.
+hipError_t launch_grouped_phased(int bm, bool stream, const Grouped& p, hipStream_t st);
 
 }  // namespace i8l

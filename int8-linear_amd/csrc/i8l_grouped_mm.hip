@@ -95,27 +95,36 @@ hipError_t launch_any_v(const Grouped& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// The rows of a tile by the rows that an expert has on average (their spread is not known here), where
-// one is faster than the next in us, over 2048 -> 1536 and 768 -> 2048 (128 experts), 2048 -> 2816 (60)
-// and 4096 -> 28672 (8), random choices, cold weights:
-//   ring 16 / 32        at 4 rows 55.1 / 57.9, 39.8 / 37.4, 45.1 / 47.2, 146 / 146; at 8 60.7 / 60.2,
-//                       44.5 / 40.8, 51.5 / 51.7, 157 / 150
-//   ring 32 / 64        at 8 60.2 / 64.4, 40.8 / 44.3, 51.7 / 53.7, 150 / 150; at 16 73.2 / 74.8,
-//                       50.0 / 50.7, 63.7 / 66.3, 165 / 157
-//   ring 64 / tile 64   at 16 74.8 / 77.1, 50.7 / 43.9, 66.3 / 68.6, 157 / 202; at 24 87.4 / 87.1,
-//                       57.9 / 50.1, 73.5 / 69.4, 167 / 205; at 48 110 / 94.6, 73.4 / 54.7, 90.0 / 76.6,
-//                       208 / 206: the ring streams the weights of a long K faster
-//   tile 64 / 128       at 48 94.6 / 95.4, 54.7 / 58.7, 76.6 / 74.6, 206 / 211; at 64 93.2 / 92.9,
-//                       61.0 / 60.4, 86.9 / 86.1, 209 / 214; at 96 114 / 100, 71.1 / 72.4, 98.2 / 92.5,
-//                       237 / 218
-//   tile 128 / 256      at 128 116 / 131, 79.1 / 85.2, 94.0 / 101, 242 / 245; at 256 165 / 161,
-//                       109 / 114, 145 / 149, 315 / 317; at 512 264 / 245, 176 / 173, 226 / 216, 523 / 517
+// The schedule, by the rows that an expert has on average (their spread is not known here).  Measured in
+// us with random choices and cold weights over 128 experts 2048 -> 1536 / 128 768 -> 2048 / 60
+// 2048 -> 2816 / 32 7168 -> 4096 / 8 4096 -> 28672 / 8 14336 -> 4096:
+//   ring of 16 rows    at 2 rows 47 / 33 / 41 / 105 / 113 / 61; of 32 49 / 32 / 42 / 104 / 114 / 62
+//   ring of 32 rows    at 8 60 / 41 / 52 / 134 / 152 / 74, of 16 61 / 45 / 52 / 144 / 157 / 90, of 64
+//                      65 / 44 / 54 / 139 / 151 / 73; at 16 74 / 50 / 64 / 152 / 165 / 96, of 64
+//                      75 / 51 / 66 / 148 / 158 / 76
+//   tile of 64 rows    at 16 70 / 42 / 64 / 146 / 176 / 100; at 32 79 / 48 / 74 / 182 / 180 / 105,
+//                      the ring of 64 95 / 62 / 82 / 178 / 176 / 84: where the tiles fill the card in
+//                      whole rounds they stream the weights as fast as the ring and multiply faster
+//                      (rounds filled: 1 / 1 / .86 / 1 / .88 / .5)
+//   tile of 128 rows   at 32 74 / 47 / 67 / 149 / 180 / 107; at 64 86 / 55 / 80 / 156 / 187 / 117, of 64
+//                      88 / 60 / 81 / 178 / 190 / 107
+//   weights kept       (tile of 128) at 64 90 / 55 / 82 / 175 / 203 / 123; at 128 105 / 73 / 86 / 205 /
+//                      228 / 125, streamed 106 / 74 / 88 / 214 / 235 / 121; at 256 156 / 105 / 139 /
+//                      299 / 306 / 211, streamed 163 / 113 / 140 / 330 / 310 / 213
+//   tile of 256 rows   at 192 142 / 90 / 116 / 256 / 235 / 155, of 128 132 / 89 / 117 / 282 / 252 / 129;
+//                      at 512 237 / 167 / 208 / 495 / 517 / 294, of 128 253 / 174 / 220 / 531 / 516 / 305
 hipError_t launch_fast(const Grouped& p, hipStream_t st) {
   const int64_t each = p.R / p.E;
   if (each < 6) return launch_grouped_ring(16, p, st);
-  if (each < 14) return launch_grouped_ring(32, p, st);
-  if (each < (p.K >= 4096 ? 44 : p.K > 1024 ? 20 : 14)) return launch_grouped_ring(64, p, st);
-  return launch_grouped_phased(each < 64 ? 64 : each < 256 ? 128 : 256, p, st);
+  const int64_t tiles = std::min(p.R, p.E) * (int64_t)((p.N + 255) / 256), cus = cu_count();
+  const int64_t room = (tiles + cus - 1) / cus * cus;   // of the rounds that the tiles take
+  const int64_t ring = 20 * tiles >= 19 * room ? 10 : 10 * tiles < 7 * room ? 44 : p.K >= 4096 ? 34 : 18;
+  if (each < ring) return launch_grouped_ring(each < 14 ? 32 : 64, p, st);
+  // (a weight row's steps share cache lines unless it starts on one)
+  const bool lines = ((uintptr_t)p.b | (uint64_t)p.eb | (uint64_t)p.ldb) % 128 == 0;
+  if (each < 24) return launch_grouped_phased(64, lines, p, st);
+  if (each < (p.K > 1024 ? 208 : 400)) return launch_grouped_phased(128, lines && each < 112, p, st);
+  return launch_grouped_phased(256, false, p, st);
 }
 
 }  // namespace

@@ -68,7 +68,8 @@ __device__ __forceinline__ T at32(const T* p, int i) {
 
 constexpr int kBadRow = -2;   // a source row outside [0, M): zeros, and NaN in the end
 
-template <int WM, int QA, int QB, int OD, bool BIAS, bool SILU>
+// STREAM: the weights are not kept in the caches, as most experts' are read by one row block only.
+template <int WM, int QA, int QB, int OD, bool BIAS, bool SILU, bool STREAM>
 __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes, uint32_t bbytes, int steps) {
   constexpr int W = 4, WN = W / WM;
   constexpr int QN = 2 * QB;                         // column fragments of a wave
@@ -198,7 +199,9 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
     copy_1k(bufA, voffA[h][j] | past, kreq, lds0 + (2 * buf + h) * HA + j * 1024 * W);
   };
   auto copyB = [&](int h, int buf, int j) {
-    copy_1k(bufB, voffB | past, kreq + brow[h][j], lds0 + B0 + buf * SB + h * HB + j * 1024 * W);
+    const uint32_t dst = lds0 + B0 + buf * SB + h * HB + j * 1024 * W;
+    if constexpr (STREAM) copy_1k_stream(bufB, voffB | past, kreq + brow[h][j], dst);
+    else copy_1k(bufB, voffB | past, kreq + brow[h][j], dst);
   };
 
   // Fragment reads: lane l reads row l%32 of a 32-row block, chunk 2*kk + l/32.
@@ -513,9 +516,9 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
 }
 
 // ------------------------------------------------------------------ host side
-template <int WM, int QA, int QB, int OD, bool BIAS, bool SILU>
+template <int WM, int QA, int QB, int OD, bool BIAS, bool SILU, bool STREAM>
 hipError_t launch_k(const Grouped& p, hipStream_t st) {
-  auto kern = grouped_phased<WM, QA, QB, OD, BIAS, SILU>;
+  auto kern = grouped_phased<WM, QA, QB, OD, BIAS, SILU, STREAM>;
   constexpr int BM = WM * 64 * QA, BN = (4 / WM) * 64 * QB;
   constexpr size_t shm = 2 * (size_t)(BM + BN) * kStep + 4 * 4096 + sizeof(PhasedShared);
   static_assert(shm <= kMaxLds, "two buffers, the staging and the tables fit the LDS");
@@ -532,13 +535,15 @@ hipError_t launch_k(const Grouped& p, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <int WM, int QA, int QB>
+template <int WM, int QA, int QB, bool STREAM>
 hipError_t launch_t(const Grouped& p, hipStream_t st) {
   auto go = [&](auto od) {
     constexpr int OD = decltype(od)::value;
     if (p.silu)
-      return p.bias ? launch_k<WM, QA, QB, OD, true, true>(p, st) : launch_k<WM, QA, QB, OD, false, true>(p, st);
-    return p.bias ? launch_k<WM, QA, QB, OD, true, false>(p, st) : launch_k<WM, QA, QB, OD, false, false>(p, st);
+      return p.bias ? launch_k<WM, QA, QB, OD, true, true, STREAM>(p, st)
+                    : launch_k<WM, QA, QB, OD, false, true, STREAM>(p, st);
+    return p.bias ? launch_k<WM, QA, QB, OD, true, false, STREAM>(p, st)
+                  : launch_k<WM, QA, QB, OD, false, false, STREAM>(p, st);
   };
   if (p.out_dtype == I8L_BF16) return go(std::integral_constant<int, I8L_BF16>{});
   if (p.out_dtype == I8L_F16) return go(std::integral_constant<int, I8L_F16>{});
@@ -547,10 +552,10 @@ hipError_t launch_t(const Grouped& p, hipStream_t st) {
 
 }  // namespace
 
-hipError_t launch_grouped_phased(int bm, const Grouped& p, hipStream_t st) {
-  if (bm == 64) return launch_t<1, 1, 1>(p, st);
-  if (bm == 128) return launch_t<2, 1, 2>(p, st);
-  return launch_t<2, 2, 2>(p, st);
+hipError_t launch_grouped_phased(int bm, bool stream, const Grouped& p, hipStream_t st) {
+  if (bm == 64) return stream ? launch_t<1, 1, 1, true>(p, st) : launch_t<1, 1, 1, false>(p, st);
+  if (bm == 128) return stream ? launch_t<2, 1, 2, true>(p, st) : launch_t<2, 1, 2, false>(p, st);
+  return launch_t<2, 2, 2, false>(p, st);
 }
 
 }  // namespace i8l
