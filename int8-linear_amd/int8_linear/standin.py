@@ -38,7 +38,7 @@ from __future__ import annotations
 import torch
 
 from int8_linear import fused_quant as fq
-from int8_linear import mxfp4
+from int8_linear import moe, mxfp4
 from int8_linear.kernel import w8a8_mm
 from int8_linear.qk_rope import qk_norm_rope, rope_cos_sin
 
@@ -250,7 +250,88 @@ class Mxfp4StandIn:
         return (h, keys) if with_keys else h
 
 
-def per_layer_us(stack: DecoderStandIn | Mxfp4StandIn, windows: int = 5, min_window_ms: float = 20.0,
+class ExpertsStandIn:
+    """The int8 decoder with its MLP split over experts: every token takes TOP_K of EXPERTS, each
+    EXPERT_INTER wide.  Attention is left out as in DecoderStandIn.  Per layer:
+
+        add_rmsnorm_quant -> qkv_proj -> quant_per_token(q columns) -> o_proj -> add_rmsnorm_quant
+        -> router (int8, fp32 logits) -> moe_route -> w8a8_grouped_mm_silu_mul -> quant_per_token
+        -> w8a8_grouped_mm -> moe_combine
+
+    The token rows are quantized once: qkv_proj's, the router's and the experts' operands are the
+    codes of the norm before them.  Operands as in DecoderStandIn, all drawn on the device (302 MB of
+    experts a layer); the route follows from them.  With first_expert and local_experts a rank's
+    share: only those experts' weights are held, and only their rows computed.
+    """
+
+    EXPERTS, TOP_K, EXPERT_INTER = 64, 8, 768
+
+    def __init__(self, m: int, layers: int = LAYERS, seed: int = 0,
+                 device: str | torch.device = "cuda", first_expert: int = 0,
+                 local_experts: int | None = None):
+        dev = torch.device(device)
+        g = torch.Generator(device=dev).manual_seed(seed)
+        self.m = m
+        self.first = first_expert
+        self.local = self.EXPERTS - first_expert if local_experts is None else local_experts
+        self.x = torch.randn((m, HIDDEN), generator=g, device=dev).to(torch.bfloat16)
+        self.norm = torch.ones(HIDDEN, dtype=torch.bfloat16, device=dev)
+        e, i = self.EXPERTS, self.EXPERT_INTER
+        mine = slice(self.first, self.first + self.local)
+        self.layers: list[dict[str, tuple[torch.Tensor, torch.Tensor]]] = []
+
+        def weight(*shape):   # the sums of products of the experts' codes stay near one
+            w = torch.randint(-127, 128, shape, generator=g, dtype=torch.int8, device=dev)
+            return w, torch.rand(shape[:-1], generator=g, device=dev) * 4e-4 + 1e-4
+        for _ in range(layers):
+            layer = {name: weight(n, k) for name, (k, n) in SHAPES.items() if name in ("qkv_proj", "o_proj")}
+            layer["router"] = weight(e, HIDDEN)
+            for name, (n, k) in (("gate_up", (2 * i, HIDDEN)), ("down", (HIDDEN, i))):
+                w, s = weight(e, n, k)
+                layer[name] = (w[mine].clone(), s[mine].clone()) if self.local < e else (w, s)
+            self.layers.append(layer)
+
+    def weight_bytes(self) -> int:
+        return sum(w.numel() + 4 * s.numel() for layer in self.layers for w, s in layer.values())
+
+    def mm(self, layer, name: str, q, s, dtype=torch.bfloat16) -> torch.Tensor:
+        w, ws = layer[name]
+        return w8a8_mm(q, w.t(), s, ws, dtype)
+
+    def route(self, logits: torch.Tensor):
+        """(weights, offsets, tokens, places): moe_route's, or its order over this rank's experts."""
+        r = moe.moe_route(logits, self.TOP_K)
+        if self.local == self.EXPERTS:
+            return r.weights, r.offsets, r.tokens, r.places
+        return r.weights, *moe.moe_order(r.experts - self.first, self.local)
+
+    def experts(self, layer, q: torch.Tensor, s: torch.Tensor, route) -> torch.Tensor:
+        """The experts' MLPs of the quantized rows, summed back to the tokens."""
+        weights, offsets, tokens, places = route
+        w, ws = layer["gate_up"]
+        out = None
+        if self.local < self.EXPERTS:   # rows of other ranks' experts are quantized too, as zeros
+            out = torch.zeros((tokens.shape[0], self.EXPERT_INTER), dtype=torch.bfloat16, device=q.device)
+        y = moe.w8a8_grouped_mm_silu_mul(q, w.transpose(1, 2), s, ws, offsets, rows=tokens, out=out)
+        q, s = fq.quant_per_token(y, fq.PRECISE_DIV)
+        w, ws = layer["down"]
+        y = moe.w8a8_grouped_mm(q, w.transpose(1, 2), s, ws, offsets)
+        return moe.moe_combine(y, weights, places)
+
+    def forward(self):
+        """One step through every layer: the last layer's MLP output [m, HIDDEN]."""
+        h, res = self.x, None
+        for layer in self.layers:
+            q, s, rout = fq.add_rmsnorm_quant(h, res, self.norm, EPS, fq.PRECISE_DIV)
+            res = h if res is None else rout
+            a = self.mm(layer, "qkv_proj", q, s)
+            h = self.mm(layer, "o_proj", *fq.quant_per_token(a[:, :Q_COLS], fq.PRECISE_DIV))
+            q, s, res = fq.add_rmsnorm_quant(h, res, self.norm, EPS, fq.PRECISE_DIV)
+            h = self.experts(layer, q, s, self.route(self.mm(layer, "router", q, s, torch.float32)))
+        return h
+
+
+def per_layer_us(stack: DecoderStandIn | Mxfp4StandIn | ExpertsStandIn, windows: int = 5, min_window_ms: float = 20.0,
                  check=None) -> float:
     """Median microseconds per decoder layer, with the whole step captured as one HIP graph
     and replayed (the reference's discipline, bench/situ_tune.py:127-154).  `check`, if
