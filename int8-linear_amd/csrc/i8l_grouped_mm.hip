@@ -115,11 +115,13 @@ hipError_t launch_any_v(const Grouped& p, hipStream_t st) {
 //                      at 512 237 / 167 / 208 / 495 / 517 / 294, of 128 253 / 174 / 220 / 531 / 516 / 305
 hipError_t launch_fast(const Grouped& p, hipStream_t st) {
   const int64_t each = p.R / p.E;
-  if (each < 6) return launch_grouped_ring(16, p, st);
+  // (a ring's grid holds all its tiles, 512 threads each, and counts those below 2^32)
+  const bool rings = (most_blocks(p.R, p.E, 16) + 32) * ((p.N + 31) / 32) < (1 << 23) - 32;
+  if (each < 6 && rings) return launch_grouped_ring(16, p, st);
   const int64_t tiles = std::min(p.R, p.E) * (int64_t)((p.N + 255) / 256), cus = cu_count();
   const int64_t room = (tiles + cus - 1) / cus * cus;   // of the rounds that the tiles take
   const int64_t ring = 20 * tiles >= 19 * room ? 10 : 10 * tiles < 7 * room ? 44 : p.K >= 4096 ? 34 : 18;
-  if (each < ring) return launch_grouped_ring(each < 14 ? 32 : 64, p, st);
+  if (each < ring && rings) return launch_grouped_ring(each < 14 ? 32 : 64, p, st);
   // (a weight row's steps share cache lines unless it starts on one)
   const bool lines = ((uintptr_t)p.b | (uint64_t)p.eb | (uint64_t)p.ldb) % 128 == 0;
   if (each < 24) return launch_grouped_phased(64, lines, p, st);
@@ -137,7 +139,7 @@ bool grouped_fast_ok(const Grouped& p) {
          p.eb % 16 == 0 && p.N % (p.silu ? 16 : 8) == 0 && aligned16(p.sb) && aligned16(p.bias) &&
          aligned16(p.out) && p.ldc * es % 16 == 0 && (int64_t)p.M * p.lda + 2 * p.K < most &&
          (int64_t)p.N * p.ldb + 2 * p.K < most && p.ldc * es < ((int64_t)1 << 22) &&
-         (most_blocks(p.R, p.E, 16) + 1) * ((p.N + 31) / 32) < (1 << 22);
+         (most_blocks(p.R, p.E, 64) + 1) * ((p.N + 127) / 128) < (1 << 30);
 }
 
 hipError_t launch_grouped_any(const Grouped& p, hipStream_t st) {

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
   const v4u bufA = buffer_of(p.a, abytes);
   v4u bufB = bufA;
   uint32_t voffA[2][JA];
-  int kreq;                // the K position being requested
+  int kreq, kat;           // the K position being requested; 0 for it past K, where nothing is read
   uint32_t past = 0;       // kOutside in the lanes whose chunk of that step lies past K
   // (found again at the start of the tile, rather than kept over the epilogue)
   auto request_from = [&](const GroupTile& g, int buf, int k) {
@@ -193,15 +193,18 @@ __global__ void __launch_bounds__(256) grouped_phased(Grouped p, uint32_t abytes
       }
     }
   };
-  auto begin_step = [&] { past = kreq + chunk < p.K ? 0u : kOutside; };
+  auto begin_step = [&] {
+    past = kreq + chunk < p.K ? 0u : kOutside;
+    kat = kreq < p.K ? kreq : 0;   // (so that the scalar offset stays within the buffer)
+  };
   // copy j of A's / B's half h of the step being requested, into buffer buf
   auto copyA = [&](int h, int buf, int j) {
-    copy_1k(bufA, voffA[h][j] | past, kreq, lds0 + (2 * buf + h) * HA + j * 1024 * W);
+    copy_1k(bufA, voffA[h][j] | past, kat, lds0 + (2 * buf + h) * HA + j * 1024 * W);
   };
   auto copyB = [&](int h, int buf, int j) {
     const uint32_t dst = lds0 + B0 + buf * SB + h * HB + j * 1024 * W;
-    if constexpr (STREAM) copy_1k_stream(bufB, voffB | past, kreq + brow[h][j], dst);
-    else copy_1k(bufB, voffB | past, kreq + brow[h][j], dst);
+    if constexpr (STREAM) copy_1k_stream(bufB, voffB | past, kat + brow[h][j], dst);
+    else copy_1k(bufB, voffB | past, kat + brow[h][j], dst);
   };
 
   // Fragment reads: lane l reads row l%32 of a 32-row block, chunk 2*kk + l/32.
