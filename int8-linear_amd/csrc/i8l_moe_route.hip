@@ -22,6 +22,9 @@
 // consecutive pieces, counted by LDS adds (sums of ones: any order) and then walked 64 pairs at a time,
 // a pair's rank among equals from ballots of the expert's bits.  No atomic decides an order, so a call's
 // results are the same every time.
+//
+// What bounds it is latency: 8192 tokens' 128 fp32 logits 7.2 us (8 rounds of dependent maxima, about 55
+// instructions each for a wave's four tokens) and 5.7 for their order; one token's bf16 logits 3.9 us in all.
 #include "i8l_common.h"
 
 #include <algorithm>
