@@ -134,12 +134,14 @@ hipError_t launch_fast(const Grouped& p, hipStream_t st) {
 }  // namespace
 
 // Offsets of 32 bits with bit 31 to spare, 16-byte pieces of every row, whole vectors of the epilogue.
+// (M counts by itself where A's rows are one row expanded: the row scales lie at 32-bit byte offsets.)
 bool grouped_fast_ok(const Grouped& p) {
   const int es = elt_size(p.out_dtype);
   const int64_t most = (int64_t)kOutside - 1024;   // (a step may be requested past K)
   return p.K % 16 == 0 && aligned16(p.a) && aligned16(p.b) && p.lda % 16 == 0 && p.ldb % 16 == 0 &&
          p.eb % 16 == 0 && p.N % (p.silu ? 16 : 8) == 0 && aligned16(p.sb) && aligned16(p.bias) &&
          aligned16(p.out) && p.ldc * es % 16 == 0 && (int64_t)p.M * p.lda + 2 * p.K < most &&
+         p.M <= 1 << 30 &&
          (int64_t)p.N * p.ldb + 2 * p.K < most && p.ldc * es < ((int64_t)1 << 22) &&
          (most_blocks(p.R, p.E, 64) + 1) * ((p.N + 127) / 128) < (1 << 30);
 }
