@@ -268,9 +268,11 @@ bool mx_plain(const at::Tensor& q, const at::Tensor& s, const at::Device& dev, i
          (r <= 1 || (q.stride(rows) >= kb && s.stride(0) >= kb / 16));
 }
 
-// Whether a floating output would lose this input's gradient: the Python way refuses the call.
+// Whether a floating output would lose this input's gradient, or its tangent in forward mode (level 0 is
+// the only one there is): the Python way refuses the call.
 bool loses_gradient(const at::Tensor& t) {
-  return at::GradMode::is_enabled() && t.defined() && t.requires_grad();
+  if (!t.defined()) return false;
+  return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined();
 }
 bool loses_gradient(const c10::optional<at::Tensor>& t) { return t.has_value() && loses_gradient(*t); }
 

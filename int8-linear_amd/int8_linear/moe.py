@@ -25,8 +25,8 @@ orders its own with moe_order (any expert outside [0, n_experts) is elsewhere); 
 offsets[n_experts] on are then not computed, and moe_combine leaves those pairs out.
 
 Launches go on the caller's current stream and allocate nothing but the outputs and, for more than
-64 tokens, the ordering's counts (up to 516 KiB).  There is no backward: what would carry a gradient
-is refused where gradients are recorded.
+64 tokens, the ordering's counts (up to 516 KiB).  There is no backward and no forward mode: what would
+carry a gradient is refused where gradients are recorded, and what has a tangent in forward mode.
 """
 
 from __future__ import annotations

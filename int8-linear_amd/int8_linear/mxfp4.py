@@ -21,13 +21,14 @@ Launches go on the caller's current stream and allocate nothing but the outputs,
 of 33 to 4096 tokens has too few tiles for the card and its K is cut into parts, the parts' sums (up to
 64 MiB; 14336 -> 4096: from 81 to 640 tokens).
 
-There is no backward.  Codes and scales are integers and carry no gradient; a call whose floating
-output would lose one is refused.
+There is no backward and no forward mode.  Codes and scales are integers and carry no gradient; a call
+whose floating output would lose one, or a tangent, is refused.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from int8_linear import _lib
 from int8_linear.fused_quant import _act_code, _fast
@@ -68,9 +69,11 @@ def _matrix(codes: torch.Tensor, scales: torch.Tensor, what: str):
 
 
 def _no_gradient(who: str, *inputs: torch.Tensor | None) -> None:
-    """Refuses inputs whose gradient a floating output of `who` would lose."""
+    """Refuses inputs whose gradient, or forward mode's tangent, a floating output of `who` would lose."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
         raise NotSupported(f"{who} has no gradient: call it under torch.no_grad()")
+    if any(t is not None and unpack_dual(t).tangent is not None for t in inputs):
+        raise NotSupported(f"{who} has no gradient: an input has a tangent")
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -275,6 +278,7 @@ def _(x, round_scale):
 def add_rmsnorm_mxfp4_quant_op(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
                                eps: float, round_scale: bool) -> tuple[torch.Tensor, torch.Tensor,
                                                                        torch.Tensor]:
+    _no_gradient("add_rmsnorm_mxfp4_quant", x, residual)   # (a copy has no tangent)
     return add_rmsnorm_mxfp4_quant(x.contiguous(), residual.contiguous(), weight, eps, round_scale)
 
 

@@ -18,6 +18,7 @@ import torch
 from int8_linear import _lib
 from int8_linear.fused_quant import _act_code, _fast
 from int8_linear.kernel import NotSupported, same_device
+from int8_linear.mxfp4 import _no_gradient
 
 _FLOAT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
 
@@ -81,14 +82,12 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     outside the table gets NaN in its rotated values.  The pairs are (i, i + rot / 2), or
     (2i, 2i + 1) with interleaved.  With inplace, q and k are written over and returned.  There is no
     backward: heads, weights or a table that require a gradient are refused where gradients are
-    recorded.
+    recorded, and those with a tangent in forward mode.
     """
     r = _fast("qk_norm_rope", q, k, q_weight, k_weight, cos_sin, positions, eps, interleaved, inplace)
     if r is not None:
         return r
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad
-                                       for x in (q, k, q_weight, k_weight, cos_sin)):
-        raise NotSupported("qk_norm_rope has no gradient: call it under torch.no_grad()")
+    _no_gradient("qk_norm_rope", q, k, q_weight, k_weight, cos_sin)
     act = _heads(q, "q", inplace)
     if _heads(k, "k", inplace) != act:
         raise NotSupported(f"q and k must have one dtype, got {q.dtype} and {k.dtype}")
