@@ -477,6 +477,12 @@ int i8l_w8a8_grouped_mm(const int8_t* a, int64_t lda, int64_t M, const int32_t* 
                         int32_t out_dtype, int32_t silu_mul, int64_t R, int64_t E, int64_t N,
                         int64_t K, void* stream);
 
+/* The tile (ordered rows x weight rows) that i8l_w8a8_grouped_mm launches for operands that meet those
+ * conditions (tile_n 64: the ring for few rows, 256: macro tiles), and whether the weights are read past
+ * the caches.  lines: the weight, expert_stride and ldb are multiples of 128 bytes.  Host-only. */
+int i8l_w8a8_grouped_mm_tile(int64_t R, int64_t E, int64_t N, int64_t K, int32_t lines,
+                             int32_t* tile_m, int32_t* tile_n, int32_t* streamed);
+
 /*
  * out[t,n] = cast((base[t,n] +) sum_j weights[t,j] * y[places[t,j],n]), j in order, in fp32, one
  * rounding.  y [R,N] (bf16/f16/f32), base (NULL: none) [T,N] and the contiguous out [T,N] of one

@@ -34,6 +34,8 @@ struct Grouped {
 
 constexpr int kMaxExperts = 512;
 constexpr int64_t kMostRows = (int64_t)1 << 25;   // (the sum of any 512 experts' blocks fits an int)
+constexpr int64_t kMostColumns = (int64_t)1 << 24;
+constexpr int64_t kMostK = (int64_t)1 << 17;   // below it the int32 sum of products of two codes cannot overflow
 
 // The most blocks of `bm` rows that R rows over E experts make.
 inline int64_t most_blocks(int64_t R, int64_t E, int bm) {

@@ -115,20 +115,30 @@ hipError_t launch_any_v(const Grouped& p, hipStream_t st) {
 //                      299 / 306 / 211, streamed 163 / 113 / 140 / 330 / 310 / 213
 //   tile of 256 rows   at 192 142 / 90 / 116 / 256 / 235 / 155, of 128 132 / 89 / 117 / 282 / 252 / 129;
 //                      at 512 237 / 167 / 208 / 495 / 517 / 294, of 128 253 / 174 / 220 / 531 / 516 / 305
-hipError_t launch_fast(const Grouped& p, hipStream_t st) {
-  const int64_t each = p.R / p.E;
+struct Schedule {
+  int bm;        // rows of a tile
+  bool ring;     // tiles of 64 columns, else of 256
+  bool stream;   // the weights past the caches
+};
+// lines: a weight's rows start on cache lines (else two of a row's steps share one).
+Schedule schedule_of(int64_t R, int64_t E, int64_t N, int64_t K, bool lines) {
+  const int64_t each = R / E;
   // (a ring's grid holds all its tiles, 512 threads each, and counts those below 2^32)
-  const bool rings = (most_blocks(p.R, p.E, 16) + 32) * ((p.N + 31) / 32) < (1 << 23) - 32;
-  if (each < 6 && rings) return launch_grouped_ring(16, p, st);
-  const int64_t tiles = std::min(p.R, p.E) * (int64_t)((p.N + 255) / 256), cus = cu_count();
+  const bool rings = (most_blocks(R, E, 16) + 32) * ((N + 31) / 32) < (1 << 23) - 32;
+  if (each < 6 && rings) return {16, true, true};
+  const int64_t tiles = std::min(R, E) * ((N + 255) / 256), cus = cu_count();
   const int64_t room = (tiles + cus - 1) / cus * cus;   // of the rounds that the tiles take
-  const int64_t ring = 20 * tiles >= 19 * room ? 10 : 10 * tiles < 7 * room ? 44 : p.K >= 4096 ? 34 : 18;
-  if (each < ring && rings) return launch_grouped_ring(each < 14 ? 32 : 64, p, st);
-  // (a weight row's steps share cache lines unless it starts on one)
+  const int64_t ring = 20 * tiles >= 19 * room ? 10 : 10 * tiles < 7 * room ? 44 : K >= 4096 ? 34 : 18;
+  if (each < ring && rings) return {each < 14 ? 32 : 64, true, true};
+  if (each < 24) return {64, false, lines};
+  if (each < (K > 1024 ? 208 : 400)) return {128, false, lines && each < 112};
+  return {256, false, false};
+}
+
+hipError_t launch_fast(const Grouped& p, hipStream_t st) {
   const bool lines = ((uintptr_t)p.b | (uint64_t)p.eb | (uint64_t)p.ldb) % 128 == 0;
-  if (each < 24) return launch_grouped_phased(64, lines, p, st);
-  if (each < (p.K > 1024 ? 208 : 400)) return launch_grouped_phased(128, lines && each < 112, p, st);
-  return launch_grouped_phased(256, false, p, st);
+  const Schedule s = schedule_of(p.R, p.E, p.N, p.K, lines);
+  return s.ring ? launch_grouped_ring(s.bm, p, st) : launch_grouped_phased(s.bm, s.stream, p, st);
 }
 
 }  // namespace
@@ -159,6 +169,23 @@ hipError_t launch_grouped_any(const Grouped& p, hipStream_t st) {
 
 using namespace i8l;
 
+extern "C" int i8l_w8a8_grouped_mm_tile(int64_t R, int64_t E, int64_t N, int64_t K, int32_t lines,
+                                        int32_t* tile_m, int32_t* tile_n, int32_t* streamed) {
+  if (!tile_m || !tile_n || !streamed) {
+    set_error("w8a8_grouped_mm_tile: an output is NULL");
+    return I8L_INVALID_ARG;
+  }
+  if (R < 0 || E < 1 || N < 0 || K < 1 || E > kMaxExperts || R > kMostRows || N > kMostColumns ||
+      K >= kMostK) {
+    set_error("w8a8_grouped_mm_tile: bad sizes R=%lld E=%lld N=%lld K=%lld", (long long)R,
+              (long long)E, (long long)N, (long long)K);
+    return I8L_INVALID_ARG;
+  }
+  const Schedule s = schedule_of(R, E, N, K, lines != 0);
+  *tile_m = s.bm, *tile_n = s.ring ? 64 : 256, *streamed = s.stream;
+  return I8L_OK;
+}
+
 extern "C" int i8l_w8a8_grouped_mm(const int8_t* a, int64_t lda, int64_t M, const int32_t* rows,
                                    const int8_t* b, int64_t expert_stride, int64_t ldb,
                                    const float* scale_a, int64_t scale_a_len, const float* scale_b,
@@ -181,9 +208,7 @@ extern "C" int i8l_w8a8_grouped_mm(const int8_t* a, int64_t lda, int64_t M, cons
               (long long)M);
     return I8L_INVALID_ARG;
   }
-  if (E > kMaxExperts || R > kMostRows || M > INT32_MAX || N > ((int64_t)1 << 24) ||
-      K >= ((int64_t)1 << 17)) {
-    // (the int32 sum of fewer than 2^17 products of two codes cannot overflow)
+  if (E > kMaxExperts || R > kMostRows || M > INT32_MAX || N > kMostColumns || K >= kMostK) {
     set_error("w8a8_grouped_mm: up to %d experts, 2^25 rows, 2^24 columns and a K below 2^17, got "
               "R=%lld E=%lld N=%lld K=%lld", kMaxExperts, (long long)R, (long long)E, (long long)N,
               (long long)K);

@@ -40,7 +40,8 @@ EXPORTS = ("i8l_w8a8_mm", "i8l_w8a8_mm_supported", "i8l_default_config", "i8l_la
            "i8l_mxfp4_dequant", "i8l_add_rmsnorm_mxfp4_quant", "i8l_silu_mul_mxfp4_quant",
            "i8l_mxfp4_mm", "i8l_mxfp4_mm_ws", "i8l_mxfp4_mm_workspace_bytes",
            "i8l_mxfp4_mm_tile", "i8l_qk_norm_rope", "i8l_moe_route", "i8l_moe_order",
-           "i8l_moe_route_workspace_bytes", "i8l_moe_order_workspace_bytes", "i8l_w8a8_grouped_mm", "i8l_moe_combine",
+           "i8l_moe_route_workspace_bytes", "i8l_moe_order_workspace_bytes", "i8l_w8a8_grouped_mm",
+           "i8l_w8a8_grouped_mm_tile", "i8l_moe_combine",
            "i8l_last_error", "i8l_version")
 
 _lib: ctypes.CDLL | None = None
@@ -106,6 +107,7 @@ def lib() -> ctypes.CDLL:
     L.i8l_moe_order_workspace_bytes.argtypes = [_I64, _I64, _I64]
     L.i8l_w8a8_grouped_mm.argtypes = [_P, _I64, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _P, _I32, _P,
                                       _P, _I64, _I32, _I32, _I64, _I64, _I64, _I64, _P]
+    L.i8l_w8a8_grouped_mm_tile.argtypes = [_I64, _I64, _I64, _I64, _I32] + [ctypes.POINTER(_I32)] * 3
     L.i8l_moe_combine.argtypes = [_P, _I64, _I64, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _I32, _P]
     for name in EXPORTS[:-2]:
         getattr(L, name).restype = ctypes.c_int
