@@ -441,8 +441,8 @@ int i8l_qk_norm_rope(const void* q, int64_t q_ts, int64_t q_hs, const void* k, i
  *   offsets [E+1]  expert e's ordered rows are offsets[e] .. offsets[e+1] - 1
  *   tokens [T*k]   the token of each ordered row; -1 from row offsets[E] on
  *   places [T,k]   the ordered row of each pair, -1 for a pair without an expert
- * Pairs of one expert keep their order (t, then choice).  E up to 512, k up to 64 and E, T*k up to
- * 2^25.  i8l_moe_order gives the order of experts picked elsewhere: any value outside [0,E) is a pair
+ * Pairs of one expert keep their order (t, then choice).  E up to 512, k up to 64 and to E, T*k up
+ * to 2^25.  i8l_moe_order gives the order of experts picked elsewhere: any value outside [0,E) is a pair
  * without an expert here.  workspace: the bytes that i8l_moe_route_workspace_bytes and
  * i8l_moe_order_workspace_bytes name (0: none is needed), 16-byte aligned, not shared by calls that
  * overlap.
@@ -465,10 +465,12 @@ int64_t i8l_moe_order_workspace_bytes(int64_t T, int64_t E, int64_t k);
  * scale_a M values or one, scale_b and bias (bf16/f16/f32, or NULL) [E,N] contiguous; out [R,N] of
  * out_dtype (bf16/f16/f32), rows ldc elements apart.  With silu_mul the first N/2 columns are gate
  * values g, the others up values u, and out [R,N/2] = cast(g / (1 + exp(-g)) * u), all in fp32.
- * Rows from offsets[E] on are left as they were.  Offsets are held within [0,R], each to
- * those before it; an r outside [0,M) gives NaN.  E up to 512, R up to 2^25, K below 2^17.  Any alignment;
- * fast where K, lda, ldb and expert_stride are multiples of 16, N of 8, and a, b, scale_b, bias and
- * out and its rows start on 16 bytes.  Nothing is allocated.
+ * Rows before offsets[0] and from offsets[E] on are left as they were.  Offsets are held within [0,R], each to
+ * those before it; an r outside [0,M) gives NaN.  E up to 512, R up to 2^25, N up to 2^24, K below
+ * 2^17, M below 2^31.  Any alignment; fast where K, lda, ldb and expert_stride are multiples of 16, N of 8
+ * (of 16 with silu_mul), a, b, scale_b, bias and out and its rows start on 16 bytes, a and one expert's
+ * weight each span less than 2^31 - 2 K - 1024 bytes, out's rows lie less than 2^22 bytes apart and M is
+ * at most 2^30.  Nothing is allocated.
  */
 int i8l_w8a8_grouped_mm(const int8_t* a, int64_t lda, int64_t M, const int32_t* rows,
                         const int8_t* b, int64_t expert_stride, int64_t ldb, const float* scale_a,
