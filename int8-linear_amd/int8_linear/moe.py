@@ -213,8 +213,8 @@ def w8a8_grouped_mm(a_q: torch.Tensor, b_q: torch.Tensor, scale_a: torch.Tensor,
     int8 [E, K, N] of a weight w_q [E, N, K], scale_b fp32 [E, N] or [E, N, 1], bias [E, N].  Expert
     e's rows are offsets[e] to offsets[e + 1] - 1 (int32 [E + 1]); row i reads a_q[rows[i]] with its
     scale, or a_q[i] without rows.  The arithmetic is w8a8_mm's, bit for bit.  `out` [R, N] (unit
-    column stride) takes the result; rows from offsets[E] on are left as they were there, and in a
-    new output hold anything.  A row outside a_q gives NaN; an offset outside [0, R] or below an earlier
+    column stride) takes the result; rows of no expert (before offsets[0], from offsets[E] on) are left as
+    they were there, and in a new output hold anything.  A row outside a_q gives NaN; an offset outside [0, R] or below an earlier
     one is held to those.  There is no backward: scales, a bias or an out that require a gradient are refused
     where gradients are recorded.
     """

@@ -164,6 +164,14 @@ def test_offsets_out_of_range_are_held(sizes, n, k, broken):
     check(p, torch.bfloat16, ends=held, offsets=torch.tensor(offsets, dtype=torch.int32, device="cuda"))
 
 
+@pytest.mark.parametrize("sizes,n,k", SCHEDULES)
+def test_rows_before_the_first_offset_are_left(sizes, n, k):
+    say(f"grouped, offsets from 5 on, {len(sizes)} experts {k} -> {n}")
+    p = problem(sizes, n, k)
+    p["offsets"] += 5
+    check(p, torch.bfloat16)
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("bias", [False, True])
 @pytest.mark.parametrize("r", [3, 30, 70, 500])
