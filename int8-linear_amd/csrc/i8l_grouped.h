@@ -116,8 +116,8 @@ __device__ __forceinline__ float row_scale(const Grouped& p, int i) {
 
 // g / (1 + exp(-g)) * u in fp32.  For a 16-bit output by the hardware's exp2 and reciprocal: the
 // rounded argument g * log2(e) makes exp(-g) off by |g| * 2^-24, 2^-17 of it at the end of the range
-// and far below the output's half step of 2^-9 or 2^-12; an fp32 output takes the accurate
-// exponential and the division.
+// and far below the output's half step of 2^-9 or 2^-12, and a reciprocal below 2^-126 (a gate under
+// -87.3) may be 0; an fp32 output takes the accurate exponential and the division.
 template <bool F32>
 __device__ __forceinline__ float silu_mul(float g, float u) {
   if constexpr (F32) {

@@ -98,8 +98,10 @@ hipError_t launch_any_v(const Grouped& p, hipStream_t st) {
 }
 
 // The schedule, by the rows that an expert has on average (their spread is not known here).  Measured in
-// us with random choices and cold weights over 128 experts 2048 -> 1536 / 128 768 -> 2048 / 60
-// 2048 -> 2816 / 32 7168 -> 4096 / 8 4096 -> 28672 / 8 14336 -> 4096:
+// us with random choices, some experts taken more than others, and two sets of weights or more in turn,
+// past what the Infinity Cache holds.  (At few rows an expert such a choice leaves some without any, whose
+// weights are not read: of 128 about 40 at 2 rows, 20 at 4.)  128 experts 2048 -> 1536 / 128 768 -> 2048 /
+// 60 2048 -> 2816 / 32 7168 -> 4096 / 8 4096 -> 28672 / 8 14336 -> 4096:
 //   ring of 16 rows    at 2 rows 47 / 33 / 41 / 105 / 113 / 61; of 32 49 / 32 / 42 / 104 / 114 / 62
 //   ring of 32 rows    at 8 60 / 41 / 52 / 134 / 152 / 74, of 16 61 / 45 / 52 / 144 / 157 / 90, of 64
 //                      65 / 44 / 54 / 139 / 151 / 73; at 16 74 / 50 / 64 / 152 / 165 / 96, of 64

@@ -40,11 +40,13 @@ namespace {
 // the power that bounds the multiplications).
 //
 // What bounds it: from about 1000 rows an expert the power, as in the dense tile (8 experts of 1024,
-// 4096 -> 28672, tiles of 256 rows: 781 us, 2.46 POP/s, clock 1.55 GHz at 67% MFMA busy); with fewer rows
-// and shorter K the epilogue (256 x 256: 6.5 us of 34 at a K of 2048, its 128 KB stored at 5.1 TB/s by all
-// CUs at a time; with SILU 7.2, exp and reciprocal) and the last round of tiles (128 experts of 512 rows,
-// 2048 -> 1536: 206 us, 2.0 POP/s; 4096 tokens' 32768 rows, 1 to 1400 an expert, with SILU 150 us, 1.37);
-// below about 100 the weight stream (32 rows of each of 128: 74 us for 403 MB, 5.4 TB/s).
+// 4096 -> 28672, tiles of 256 rows: 781 us, 2.46 POP/s, clock 1.55 GHz at 67% MFMA busy).  With fewer rows
+// and shorter K, that a CU holds one workgroup and a SIMD one wave, so that nothing multiplies during an
+// epilogue (256 x 256: 6.5 us of 34 at a K of 2048, its 128 KB stored at 5.1 TB/s by all CUs at a time; with
+// SILU 7.2, exp and reciprocal): 128 experts of 512 rows, 2048 -> 1536, 206 us, 2.0 POP/s.  4096 tokens'
+// 32768 rows, 1 to 1400 an expert, with SILU: 148 us, 1.4 POP/s, MFMA busy 40%; a fifth of the rows it
+// multiplies are an expert's last tile's padding, and an even deal of the tiles to workgroups won 1% of it.
+// Below about 100 rows the weight stream (32 rows of each of 128: 72 us for 403 MB, 5.6 TB/s).
 constexpr int kStep = 128;
 
 constexpr int kTiles = 32;   // found half of them at a time, a tile a lane

@@ -16,9 +16,10 @@ namespace {
 //
 // What bounds it is the weight stream: a weight byte is copied by one workgroup only (by one for each
 // 16 MT rows of its expert), and the slots of two workgroups fill a CU's LDS, so that about 140 KiB are
-// in flight a CU and one workgroup's start and end lie under the other's stream.  Cold weights: 512 rows
-// over 128 experts (2048 -> 1536, about 380 MB) 55 us, 7 TB/s; 4 tokens through 14 of 60 experts
-// (2048 -> 2816, 82 MB) 16.8; one token's 8 experts (768 -> 2048, 12.6 MB) 5.2.
+// in flight a CU and one workgroup's start and end lie under the other's stream.  Sets of weights in turn
+// / after a read of 3 GiB: 4 rows of each of 128 experts (2048 -> 1536, 403 MB) 62 / 63 us, 6.5 TB/s;
+// 4 tokens through 14 of 60 experts (2048 -> 2816, SILU, 81 MB) 17.2 / 18.0; one token's 8 experts
+// (768 -> 2048, 12.6 MB) 5.2 / 6.2.
 //
 // The start is a chain of dependent reads (offsets, then the rows' indices, then the operands), so the
 // weights are requested as soon as the tile is found and the indices come through the scalar cache,
